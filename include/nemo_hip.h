@@ -252,6 +252,52 @@ int nemo_solve_static(nemo_ctx *ctx, int32_t N, const int32_t *d_img_idx, const 
                       const float *d_feat, const float *d_clu, const float *d_C0, const float *d_theta0,
                       float *d_pose, float *d_loss, float *d_trace, int32_t *d_status, void *stream);
 
+/* ---- rows held in 8 bits ---------------------------------------------------
+ * A feature map of 80 x 100 x 128 is 4.1 MB in f32 and a quarter of that held like this, in a resident cache, in a record on
+ * disk and on its way to the GPU; no counterpart in the reference.  A row of C channels (a pixel's features, a bank row) is
+ *   codes u8[C]               e4m3 (no infinities, 0x7f / 0xff = NaN), and
+ *   scales u8[ceil(C / 128)]  one per block of 128 channels (the last block may be shorter): the byte b stands for 2^(b - 127),
+ * number = code * scale.  Quantising takes per block the smallest power of two 2^e, e >= -117, with
+ * max |x| <= 448 * 2^e over the block's finite numbers, and rounds x * 2^-e to the nearest code, ties to even: half an e4m3 step,
+ * 2^-4 of the number, or 2^-10 * 2^e where that is more.  Numbers that are not finite become NaN and leave the others alone.
+ * C is a multiple of 16 from 16 to 65536.  16-byte aligned buffers (scales: any).  No workspaces: these calls may run on several streams
+ * at once and be captured; they launch on the context's device, whichever is current.  Nothing here has a gradient. */
+#define NEMO_F32 0
+#define NEMO_BF16 1
+#define NEMO_F16 2
+
+/* Writes n images of `rows` pixels into a cache of n_slots images: image i to slot d_slots[i] (NULL: slot i).  d_x is of `dtype`
+ * [n][rows][C], or [n][C][rows] with channel_major (what a backbone leaves and a feature record holds).  d_q u8[n_slots][rows][C],
+ * d_e u8[n_slots][rows][ceil(C / 128)].  An image whose slot is outside [0, n_slots) is not written; of several images
+ * with the same slot the last one stays; slots that no image names are left as they were.  Plain rows (a bank): n = 1, rows = their number. */
+int nemo_quantize(nemo_ctx *ctx, const void *d_x, int32_t dtype, int32_t channel_major, int32_t n, int32_t rows, int32_t C,
+                  const int32_t *d_slots, int32_t n_slots, uint8_t *d_q, uint8_t *d_e, void *stream);
+/* Reads images back: slot d_slots[i] (NULL: slot i) to image i of d_x, of `dtype` and layout as above, rounded once to `dtype` (a number
+ * within half a step of 2^128 reads back as infinity); the same slot may be read several times.  An image whose slot is outside [0, n_slots) reads zeros. */
+int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const int32_t *d_slots, int32_t n_slots, int32_t n,
+                    int32_t rows, int32_t C, int32_t dtype, int32_t channel_major, void *d_x, void *stream);
+
+/* d_out[m][n] = <row m of a, row n of b> (the numbers the rows stand for), f32 or bf16 [M][N], accumulated in fp32 on the bf16 matrix
+ * cores (the numbers are exact in bf16): features against a vertex or clutter bank, or the 1x1 convolution behind a backbone. */
+int nemo_q8_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be,
+                    int32_t N, int32_t K, int32_t out_dtype, void *d_out, void *stream);
+/* The same with a bank for each segment of rows: rows d_row_off[s] .. d_row_off[s + 1] of a (i32[n_seg + 1], not decreasing, from
+ * [0, M]) times rows d_bank_off[g] .. d_bank_off[g + 1] of b (i32[n_banks + 1], not decreasing, from [0, N]), g = d_bank_of[s] (i32[n_seg];
+ * NULL: g = s, or 0 with one bank).  d_out [M][n_cols]: column j of a row is its product with row j of its bank; columns from the bank's
+ * length on, rows of no segment and rows whose d_bank_of is outside [0, n_banks) are left as they were, bank rows from n_cols on are
+ * not used.  Segments and banks may be empty. */
+int nemo_q8_grouped_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const int32_t *d_row_off, int32_t n_seg,
+                            const uint8_t *d_b, const uint8_t *d_be, int32_t N, const int32_t *d_bank_off, int32_t n_banks,
+                            const int32_t *d_bank_of, int32_t K, int32_t out_dtype, int32_t n_cols, void *d_out, void *stream);
+/* nemo_clutter_score on maps and banks held in 8 bits, with a bank per image (code/MeshPoseSolveAll.py:203-207 reads `clutter_<subtype>`
+ * inside the subtype loop): d_out f32[n_img][h][w] = max over the rows of bank d_bank_of[i] of <row, feature>.  d_feat u8[n_img][h][w][D]
+ * and its scales; d_cbank u8[K][D], its rows cut into banks by d_bank_off i32[n_banks + 1] (NULL: one bank); d_bank_of i32[n_img]
+ * (NULL: bank i, or 0 with one bank).  -infinity for an empty bank, NaN where a product is NaN; images whose d_bank_of is outside
+ * [0, n_banks) are left as they were. */
+int nemo_q8_clutter_score(nemo_ctx *ctx, const uint8_t *d_feat, const uint8_t *d_feat_e, int32_t n_img, const uint8_t *d_cbank,
+                          const uint8_t *d_cbank_e, int32_t K, const int32_t *d_bank_off, int32_t n_banks, const int32_t *d_bank_of,
+                          float *d_out, void *stream);
+
 /* Bytes the fused kernels read per covered pixel and step: 4*D + 4. */
 int64_t nemo_bytes_per_covered_pixel(const nemo_ctx *ctx);
 

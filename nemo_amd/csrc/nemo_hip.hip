@@ -1,6 +1,6 @@
 // nemo_hip.hip -- hand-written CDNA4 (gfx950) kernels + C ABI of libnemo_hip.so.  One translation unit: the device
-// code is in device_common.hpp, eval_pose.hpp, pose_kernels.hpp and matrix_kernels.hpp (included below, in that
-// order), the context, launch logic and the extern "C" entry points are here.
+// code is in device_common.hpp, eval_pose.hpp, pose_kernels.hpp, matrix_kernels.hpp and q8_kernels.hpp (included below,
+// in that order), the context, launch logic and the extern "C" entry points are here.
 //
 // One workgroup (1024 threads = 16 wave64, the CU's whole LDS) owns one job (image, mesh) and runs the
 // whole render-and-compare evaluation out of LDS (eval_pose):
@@ -39,6 +39,7 @@
 #include "eval_pose.hpp"
 #include "pose_kernels.hpp"
 #include "matrix_kernels.hpp"
+#include "q8_kernels.hpp"
 
 
 // ==================================================================== C ABI
@@ -1150,6 +1151,166 @@ int nemo_solve_table_stats(nemo_ctx *ctx, int32_t *mode, uint64_t *blocks) {
   HIP_TRY(ctx, hipMemcpy(&v, ctx->d_counter + 1, sizeof(u64), hipMemcpyDeviceToHost));
   *mode = ctx->last_solve_mode;
   *blocks = v;
+  return NEMO_OK;
+}
+
+// ---- rows held in 8 bits (q8_kernels.hpp).  No workspace, no state of the context but its error text: calls on several streams
+// do not disturb each other.
+
+// Launches go to the context's device, whichever is current.
+struct DeviceGuard {
+  int before = -1;
+  hipError_t status;
+  explicit DeviceGuard(int device) {
+    status = hipGetDevice(&before);
+    if (status == hipSuccess && before != device) status = hipSetDevice(device);
+    else before = -1;  // nothing to restore
+  }
+  ~DeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
+};
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+constexpr size_t Q8_MAX_BLOCKS = (1u << 24) - 1;  // 256 threads each: a launch holds fewer than 2^32 threads
+
+static int q8_check_rows(nemo_ctx *ctx, const char *who, int32_t dtype, int32_t n, int32_t rows, int32_t C, int32_t n_slots, const void *d_x,
+                         const void *d_q, const void *d_e) {
+  if (dtype != NEMO_F32 && dtype != NEMO_BF16 && dtype != NEMO_F16) return fail(ctx, NEMO_ERR_ARG, "%s: unknown type %d", who, dtype);
+  if (n < 0 || rows < 0 || n_slots < 0) return fail(ctx, NEMO_ERR_ARG, "%s: negative size", who);
+  if (C < 16 || C > 65536 || C % 16) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %d channels (a multiple of 16, 16 to 65536)", who, C);
+  if (n == 0 || rows == 0) return NEMO_OK;
+  if (!d_x || !d_q || !d_e) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);
+  if (!aligned16(d_x) || !aligned16(d_q)) return fail(ctx, NEMO_ERR_ARG, "%s: buffers must be 16-byte aligned", who);
+  return NEMO_OK;
+}
+
+int nemo_quantize(nemo_ctx *ctx, const void *d_x, int32_t dtype, int32_t channel_major, int32_t n, int32_t rows, int32_t C, const int32_t *d_slots,
+                  int32_t n_slots, uint8_t *d_q, uint8_t *d_e, void *stream) {
+  if (!ctx) return fail(nullptr, NEMO_ERR_ARG, "nemo_quantize: null ctx");
+  const int rc = q8_check_rows(ctx, "nemo_quantize", dtype, n, rows, C, n_slots, d_x, d_q, d_e);
+  if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
+  const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
+  const size_t per = channel_major ? ((size_t)rows + 63) / 64 : ((size_t)rows * nb + 16 * Q8_QU - 1) / (16 * Q8_QU);
+  const size_t blocks = per * (channel_major ? nb : 1) * n;
+  if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_quantize: too many rows for one launch");
+  DeviceGuard on(ctx->device);
+  HIP_TRY(ctx, on.status);
+#define Q8_LAUNCH(TT)                                                                                                             \
+  if (channel_major)                                                                                                              \
+    hipLaunchKernelGGL((q8_quantize_t_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const TT::T *)d_x, n, rows, C, nb, \
+                       (unsigned)per, d_slots, n_slots, d_q, d_e);                                                               \
+  else                                                                                                                            \
+    hipLaunchKernelGGL((q8_quantize_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const TT::T *)d_x, n, rows, C, nb, \
+                       (unsigned)per, d_slots, n_slots, d_q, d_e)
+  if (dtype == NEMO_F32) { Q8_LAUNCH(Q8F32); } else if (dtype == NEMO_BF16) { Q8_LAUNCH(Q8BF16); } else { Q8_LAUNCH(Q8F16); }
+#undef Q8_LAUNCH
+  HIP_TRY(ctx, hipGetLastError());
+  return NEMO_OK;
+}
+
+int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const int32_t *d_slots, int32_t n_slots, int32_t n, int32_t rows, int32_t C,
+                    int32_t dtype, int32_t channel_major, void *d_x, void *stream) {
+  if (!ctx) return fail(nullptr, NEMO_ERR_ARG, "nemo_dequantize: null ctx");
+  const int rc = q8_check_rows(ctx, "nemo_dequantize", dtype, n, rows, C, n_slots, d_x, d_q, d_e);
+  if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
+  const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
+  const size_t per = channel_major ? ((size_t)rows + 63) / 64 : ((size_t)rows * (C / 4) + 256 * Q8_DU - 1) / (256 * Q8_DU);
+  const size_t blocks = per * (channel_major ? nb : 1) * n;
+  if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_dequantize: too many rows for one launch");
+  DeviceGuard on(ctx->device);
+  HIP_TRY(ctx, on.status);
+#define Q8_LAUNCH(TT)                                                                                                             \
+  if (channel_major)                                                                                                              \
+    hipLaunchKernelGGL((q8_dequantize_t_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, d_e, rows, C, nb, (unsigned)per, \
+                       d_slots, n_slots, (TT::T *)d_x);                                                                          \
+  else                                                                                                                            \
+    hipLaunchKernelGGL((q8_dequantize_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, d_e, rows, C, nb, (unsigned)per, \
+                       d_slots, n_slots, (TT::T *)d_x)
+  if (dtype == NEMO_F32) { Q8_LAUNCH(Q8F32); } else if (dtype == NEMO_BF16) { Q8_LAUNCH(Q8BF16); } else { Q8_LAUNCH(Q8F16); }
+#undef Q8_LAUNCH
+  HIP_TRY(ctx, hipGetLastError());
+  return NEMO_OK;
+}
+
+// What the three products share: checks of both operands and of the segments, and the kernels' arguments.
+static int q8_operands(nemo_ctx *ctx, const char *who, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be,
+                       int32_t N, int32_t K, const void *d_out, Q8Args *A) {
+  if (M < 0 || N < 0) return fail(ctx, NEMO_ERR_ARG, "%s: negative size", who);
+  if (M > 0x7fffffff) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %lld rows (at most 2^31 - 1)", who, (long long)M);
+  if (K < 16 || K > 65536 || K % 16) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %d channels (a multiple of 16, 16 to 65536)", who, K);
+  if (M > 0 && (!d_a || !d_ae)) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);
+  if (N > 0 && (!d_b || !d_be)) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);
+  if (!aligned16(d_a) || !aligned16(d_b) || !aligned16(d_out)) return fail(ctx, NEMO_ERR_ARG, "%s: buffers must be 16-byte aligned", who);
+  memset(A, 0, sizeof(*A));
+  A->a = d_a; A->ae = d_ae; A->b = d_b; A->be = d_be;
+  A->M = (int)M; A->N = N; A->K = K; A->nb = (K + Q8_BLOCK - 1) / Q8_BLOCK;
+  return NEMO_OK;
+}
+
+static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, size_t tiles, int32_t out_dtype, void *d_out, void *stream) {
+  const size_t cols = ((size_t)A.n_cols + 31) / 32;
+  if (tiles > Q8_MAX_BLOCKS || cols > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+  DeviceGuard on(ctx->device);
+  HIP_TRY(ctx, on.status);
+  const dim3 grid((unsigned)tiles, (unsigned)cols);
+  if (out_dtype == NEMO_F32) hipLaunchKernelGGL((q8_product_kernel<Q8F32>), grid, dim3(256), 0, (hipStream_t)stream, A, (float *)d_out);
+  else hipLaunchKernelGGL((q8_product_kernel<Q8BF16>), grid, dim3(256), 0, (hipStream_t)stream, A, (uint16_t *)d_out);
+  HIP_TRY(ctx, hipGetLastError());
+  return NEMO_OK;
+}
+
+int nemo_q8_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be, int32_t N, int32_t K,
+                    int32_t out_dtype, void *d_out, void *stream) {
+  if (!ctx) return fail(nullptr, NEMO_ERR_ARG, "nemo_q8_product: null ctx");
+  if (out_dtype != NEMO_F32 && out_dtype != NEMO_BF16) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_product: the result is f32 or bf16");
+  Q8Args A;
+  const int rc = q8_operands(ctx, "nemo_q8_product", d_a, d_ae, M, d_b, d_be, N, K, d_out, &A);
+  if (rc != NEMO_OK || M == 0 || N == 0) return rc;
+  if (!d_out) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_product: null buffer");
+  A.seg_rows = A.M;
+  A.n_seg = A.n_banks = 1;
+  A.n_cols = N;
+  return q8_launch_product(ctx, "nemo_q8_product", A, ((size_t)M + 127) / 128, out_dtype, d_out, stream);
+}
+
+int nemo_q8_grouped_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const int32_t *d_row_off, int32_t n_seg,
+                            const uint8_t *d_b, const uint8_t *d_be, int32_t N, const int32_t *d_bank_off, int32_t n_banks, const int32_t *d_bank_of,
+                            int32_t K, int32_t out_dtype, int32_t n_cols, void *d_out, void *stream) {
+  if (!ctx) return fail(nullptr, NEMO_ERR_ARG, "nemo_q8_grouped_product: null ctx");
+  if (out_dtype != NEMO_F32 && out_dtype != NEMO_BF16) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_grouped_product: the result is f32 or bf16");
+  if (n_seg < 0 || n_banks < 0 || n_cols < 0) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_grouped_product: negative size");
+  Q8Args A;
+  const int rc = q8_operands(ctx, "nemo_q8_grouped_product", d_a, d_ae, M, d_b, d_be, N, K, d_out, &A);
+  if (rc != NEMO_OK || M == 0 || N == 0 || n_seg == 0 || n_banks == 0 || n_cols == 0) return rc;
+  if (!d_out) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_grouped_product: null buffer");
+  if (!d_row_off || !d_bank_off) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_grouped_product: null offsets");
+  if (!d_bank_of && n_banks != 1 && n_banks != n_seg)
+    return fail(ctx, NEMO_ERR_ARG, "nemo_q8_grouped_product: %d segments, %d banks and no d_bank_of", n_seg, n_banks);
+  A.row_off = d_row_off; A.bank_off = d_bank_off; A.bank_of = d_bank_of;
+  A.n_seg = n_seg; A.n_banks = n_banks;
+  A.n_cols = n_cols;
+  return q8_launch_product(ctx, "nemo_q8_grouped_product", A, ((size_t)M + 127) / 128 + n_seg, out_dtype, d_out, stream);
+}
+
+int nemo_q8_clutter_score(nemo_ctx *ctx, const uint8_t *d_feat, const uint8_t *d_feat_e, int32_t n_img, const uint8_t *d_cbank, const uint8_t *d_cbank_e,
+                          int32_t K, const int32_t *d_bank_off, int32_t n_banks, const int32_t *d_bank_of, float *d_out, void *stream) {
+  if (!ctx) return fail(nullptr, NEMO_ERR_ARG, "nemo_q8_clutter_score: null ctx");
+  if (n_img < 0 || n_banks < 1) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_clutter_score: bad argument");
+  const int hw = ctx->cfg.win_h * ctx->cfg.win_w;
+  Q8Args A;
+  const int rc = q8_operands(ctx, "nemo_q8_clutter_score", d_feat, d_feat_e, (int64_t)n_img * hw, d_cbank, d_cbank_e, K, ctx->cfg.feat_dim, d_out, &A);
+  if (rc != NEMO_OK || n_img == 0) return rc;
+  if (!d_out) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_clutter_score: null buffer");
+  if (!d_bank_off && n_banks != 1) return fail(ctx, NEMO_ERR_ARG, "nemo_q8_clutter_score: null offsets");
+  if (!d_bank_of && n_banks != 1 && n_banks != n_img)
+    return fail(ctx, NEMO_ERR_ARG, "nemo_q8_clutter_score: %d images, %d banks and no d_bank_of", n_img, n_banks);
+  A.seg_rows = hw;
+  A.n_seg = n_img; A.n_banks = n_banks;
+  A.bank_off = d_bank_off; A.bank_of = d_bank_of;
+  const size_t blocks = (size_t)n_img * (((size_t)hw + 127) / 128);
+  if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_q8_clutter_score: too many pixels for one launch");
+  DeviceGuard on(ctx->device);
+  HIP_TRY(ctx, on.status);
+  hipLaunchKernelGGL(q8_score_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, A, d_out);
+  HIP_TRY(ctx, hipGetLastError());
   return NEMO_OK;
 }
 

@@ -1,0 +1,428 @@
+// q8_kernels.hpp -- feature rows held in 8 bits: quantise, read back, products on the bf16 matrix cores, clutter score
+// Part of the single translation unit nemo_hip.hip (included from there, in order; not a stand-alone header).
+//
+// A row of C channels is C codes (e4m3, the format without infinities) and one scale byte per block of 128 channels:
+//   amax = the largest |x_c| of the block's finite numbers,  e = max(-117, ceil(log2(amax / 448))),
+//   code_c = e4m3(x_c 2^-e) to nearest even (NaN where x_c is not finite),  byte = e + 127.
+// The scale is a power of two because nothing is lost by it that amax / 448 would keep, but for range at the small end
+// (e4m3's step is relative), while x 2^-e and code 2^e become exact, the latter in bf16 too: 4 significant bits and fp32's range.
+// -117: the smallest code, 2^-9, times 2^-117 is still a normal number.
+//
+// Products run on the bf16 matrix instructions, on the numbers that the codes stand for (v_cvt_scalef32_pk_bf16_fp8, exact).
+// The 8-bit matrix instructions have twice the rate, but add neighbouring products after cutting each at 2^-14 of the
+// largest among them (measured; 1.4e-5 of the result where the bf16 ones are off by 5e-9): that is no fp32 sum.
+#ifndef Q8_KERNELS_HPP
+#define Q8_KERNELS_HPP
+
+namespace {
+
+constexpr int Q8_BLOCK = 128;  // channels per scale
+constexpr uint32_t Q8_INF = 0x7f800000u;
+
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef uint32_t u4va __attribute__((ext_vector_type(4)));
+
+// e of a block from the bits of its (finite) amax: 448 = 1.75 * 2^8
+__device__ __forceinline__ int q8_exponent(uint32_t amax) {
+  const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(e, -117);
+}
+__device__ __forceinline__ float q8_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+// the number a scale byte stands for (byte 0: 2^-127, byte 255: NaN; quantising writes neither)
+__device__ __forceinline__ float q8_scale(uint32_t byte) {
+  return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+}
+__device__ __forceinline__ uint32_t q8_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// four numbers, already times 2^-e, to four codes
+__device__ __forceinline__ uint32_t q8_pack(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+__device__ __forceinline__ void q8_unpack(uint32_t codes, float s, float *x) {
+  auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  x[0] = lo[0] * s; x[1] = lo[1] * s; x[2] = hi[0] * s; x[3] = hi[1] * s;
+}
+
+// the three types a row is quantised from and read back to
+struct Q8F32 { typedef float T; static __device__ __forceinline__ float get(float x) { return x; } static __device__ __forceinline__ float put(float x) { return x; } };
+struct Q8BF16 {
+  typedef uint16_t T;
+  static __device__ __forceinline__ float get(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+  static __device__ __forceinline__ uint16_t put(float x) {  // nearest even
+    const uint32_t u = __float_as_uint(x);
+    return (u & 0x7fffffffu) > Q8_INF ? (uint16_t)0x7fc0 : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+  }
+};
+struct Q8F16 {
+  typedef _Float16 T;
+  static __device__ __forceinline__ float get(_Float16 x) { return (float)x; }
+  static __device__ __forceinline__ _Float16 put(float x) { return (_Float16)x; }
+};
+
+// Where image i of a call sits in the cache: slots[i], or i.  -1: nowhere (out of range).
+__device__ __forceinline__ int q8_slot(const int32_t *slots, int i, int n_slots) {
+  const int s = slots ? slots[i] : i;
+  return s >= 0 && s < n_slots ? s : -1;
+}
+// Two images written to the same slot: the later one stays, as if they were written in order.  Whether a later image
+// than i has slot s (whole workgroup).
+__device__ __forceinline__ bool q8_overwritten(const int32_t *slots, int i, int n, int s) {
+  if (!slots) return false;
+  bool hit = false;
+  for (int j = i + 1 + (int)threadIdx.x; j < n; j += (int)blockDim.x) hit |= slots[j] == s;
+  return __syncthreads_or(hit) != 0;
+}
+
+// ---------------------------------------------------------------- quantise, channels contiguous
+// x [n][rows][C] -> q [slot][rows][C], e [slot][rows][nb].  16 lanes own a block of 128 channels, 8 numbers a lane (fp32: 4
+// in either half of the block, so that every load instruction reads whole cache lines), its maximum goes through four
+// rotations inside the 16 lanes.
+constexpr int Q8_QU = 4;  // blocks per 16 lanes: their loads are all in flight before the first is used
+template <class TT>
+__global__ __launch_bounds__(256) void q8_quantize_kernel(const typename TT::T *__restrict__ x, int n, int rows, int C, int nb, unsigned chunks,
+                                                          const int32_t *__restrict__ slots, int n_slots, uint8_t *__restrict__ q,
+                                                          uint8_t *__restrict__ e) {
+  constexpr bool F32 = sizeof(typename TT::T) == 4;
+  const int img = (int)(blockIdx.x / chunks);
+  const unsigned chunk = blockIdx.x - (unsigned)img * chunks;
+  const int slot = q8_slot(slots, img, n_slots);
+  if (slot < 0 || q8_overwritten(slots, img, n, slot)) return;
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const size_t blocks = (size_t)rows * nb, b0 = (size_t)chunk * (16 * Q8_QU) + group;
+  float v[Q8_QU][8];
+#pragma unroll
+  for (int u = 0; u < Q8_QU; ++u) {
+    const size_t blk = b0 + 16 * u;
+    const size_t row = nb == 1 ? blk : blk / nb;
+    const int c0 = nb == 1 ? 0 : (int)(blk - row * nb) * Q8_BLOCK;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + (F32 ? 64 * h + 4 * lane : 8 * lane + 4 * h);
+      const bool in = blk < blocks && c < C;
+      const typename TT::T *p = x + ((size_t)img * rows + (in ? row : 0)) * C + (in ? c : 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[u][4 * h + k] = in ? TT::get(p[k]) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < Q8_QU; ++u) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, q8_abs_bits(v[u][k]));
+    auto all16 = [](uint32_t a) {
+      a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x128, 0xf, 0xf, false));
+      a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x124, 0xf, 0xf, false));
+      a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x122, 0xf, 0xf, false));
+      return max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x121, 0xf, 0xf, false));
+    };
+    m = all16(m);
+    if (__any(m >= Q8_INF)) {  // numbers that are not finite: rare, the whole wave takes the maximum again without them
+      m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t a = q8_abs_bits(v[u][k]);
+        m = max(m, a < Q8_INF ? a : 0u);
+        v[u][k] = a < Q8_INF ? v[u][k] : __uint_as_float(0x7fc00000u);
+      }
+      m = all16(m);
+    }
+    const int ex = q8_exponent(m);
+    const float s = q8_pow2(-ex);
+    const size_t blk = b0 + 16 * u;
+    if (blk >= blocks) continue;
+    const size_t row = nb == 1 ? blk : blk / nb;
+    const int b = nb == 1 ? 0 : (int)(blk - row * nb);
+    uint8_t *qp = q + ((size_t)slot * rows + row) * C + (size_t)b * Q8_BLOCK;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = F32 ? 64 * h + 4 * lane : 8 * lane + 4 * h;
+      if (b * Q8_BLOCK + c < C) *(uint32_t *)(qp + c) = q8_pack(v[u][4 * h] * s, v[u][4 * h + 1] * s, v[u][4 * h + 2] * s, v[u][4 * h + 3] * s);
+    }
+    if (lane == 0) e[((size_t)slot * rows + row) * nb + b] = (uint8_t)(ex + 127);
+  }
+}
+
+// ---------------------------------------------------------------- quantise, pixels contiguous
+// x [n][C][rows] -> the same q and e (the layout a backbone leaves and a feature record holds).  A workgroup owns 64 pixels and one
+// block of 128 channels, a wave 32 of the channels: a lane's 32 numbers are of one pixel, so the maximum needs one exchange
+// between the waves; the codes go through LDS so that a pixel's 128 bytes leave as one line.
+template <class TT>
+__global__ __launch_bounds__(256) void q8_quantize_t_kernel(const typename TT::T *__restrict__ x, int n, int rows, int C, int nb, unsigned tiles,
+                                                            const int32_t *__restrict__ slots, int n_slots, uint8_t *__restrict__ q,
+                                                            uint8_t *__restrict__ e) {
+  __shared__ uint32_t top[4][64];
+  __shared__ __align__(16) uint8_t codes[64][Q8_BLOCK + 16];
+  const unsigned per = tiles * (unsigned)nb;
+  const int img = (int)(blockIdx.x / per);
+  const unsigned rest = blockIdx.x - (unsigned)img * per;
+  const int b = (int)(rest / tiles), p0 = (int)(rest - (unsigned)b * tiles) * 64;
+  const int slot = q8_slot(slots, img, n_slots);
+  if (slot < 0 || q8_overwritten(slots, img, n, slot)) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c0 = b * Q8_BLOCK + 32 * w, p = min(p0 + lane, rows - 1);
+  const typename TT::T *xp = x + (size_t)img * C * rows + p;
+  float v[32];
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = c0 + k < C ? TT::get(xp[(size_t)(c0 + k) * rows]) : 0.0f;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) m = max(m, q8_abs_bits(v[k]));
+  if (__any(m >= Q8_INF)) {
+    m = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const uint32_t a = q8_abs_bits(v[k]);
+      m = max(m, a < Q8_INF ? a : 0u);
+      v[k] = a < Q8_INF ? v[k] : __uint_as_float(0x7fc00000u);
+    }
+  }
+  top[w][lane] = m;
+  __syncthreads();
+  m = max(max(top[0][lane], top[1][lane]), max(top[2][lane], top[3][lane]));
+  const int ex = q8_exponent(m);
+  const float s = q8_pow2(-ex);
+#pragma unroll
+  for (int k = 0; k < 32; k += 16) {
+    u4va c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = q8_pack(v[k + 4 * j] * s, v[k + 4 * j + 1] * s, v[k + 4 * j + 2] * s, v[k + 4 * j + 3] * s);
+    *(u4va *)&codes[lane][32 * w + k] = c;
+  }
+  __syncthreads();
+  const size_t row0 = (size_t)slot * rows + p0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = (int)threadIdx.x + 256 * j, r = i >> 3, c = (i & 7) * 16;
+    if (p0 + r < rows && b * Q8_BLOCK + c < C) *(u4va *)(q + (row0 + r) * C + (size_t)b * Q8_BLOCK + c) = *(const u4va *)&codes[r][c];
+  }
+  if (w == 0 && p0 + lane < rows) e[(row0 + lane) * nb + b] = (uint8_t)(ex + 127);
+}
+
+// ---------------------------------------------------------------- read back, channels contiguous
+// q [slot][rows][C], e -> x [n][rows][C]; a lane reads 4 codes and writes 4 numbers, Q8_DU times.  An image without a slot reads zeros.
+constexpr int Q8_DU = 4;
+template <class TT>
+__global__ __launch_bounds__(256) void q8_dequantize_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ e, int rows, int C, int nb,
+                                                            unsigned chunks, const int32_t *__restrict__ slots, int n_slots,
+                                                            typename TT::T *__restrict__ x) {
+  typedef typename TT::T v4 __attribute__((ext_vector_type(4)));
+  const int img = (int)(blockIdx.x / chunks);
+  const unsigned chunk = blockIdx.x - (unsigned)img * chunks;
+  const int slot = q8_slot(slots, img, n_slots);
+  const size_t quads = (size_t)rows * (C / 4), base = (size_t)max(slot, 0) * rows;
+  const unsigned qpr = (unsigned)C / 4;  // quads per row
+#pragma unroll
+  for (int u = 0; u < Q8_DU; ++u) {
+    const size_t i = (size_t)chunk * (256 * Q8_DU) + 256 * u + threadIdx.x;
+    if (i >= quads) return;
+    const size_t row = i / qpr;
+    const unsigned c4 = (unsigned)(i - row * qpr);
+    float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (slot >= 0) q8_unpack(*(const uint32_t *)(q + base * C + 4 * i), q8_scale(e[(base + row) * nb + c4 / 32]), f);
+    v4 o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = TT::put(f[k]);
+    *(v4 *)(x + (size_t)img * rows * C + 4 * i) = o;
+  }
+}
+
+// ---------------------------------------------------------------- read back, pixels contiguous
+// q [slot][rows][C], e -> x [n][C][rows]: 64 pixels x 128 channels through LDS.
+template <class TT>
+__global__ __launch_bounds__(256) void q8_dequantize_t_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ e, int rows, int C, int nb,
+                                                              unsigned tiles, const int32_t *__restrict__ slots, int n_slots,
+                                                              typename TT::T *__restrict__ x) {
+  __shared__ uint32_t codes[64][Q8_BLOCK / 4 + 1];
+  const unsigned per = tiles * (unsigned)nb;
+  const int img = (int)(blockIdx.x / per);
+  const unsigned rest = blockIdx.x - (unsigned)img * per;
+  const int b = (int)(rest / tiles), p0 = (int)(rest - (unsigned)b * tiles) * 64;
+  const int slot = q8_slot(slots, img, n_slots);
+  const size_t row0 = (size_t)max(slot, 0) * rows + p0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = (int)threadIdx.x + 256 * j, r = i >> 5, c = i & 31;
+    uint32_t v = 0;
+    if (slot >= 0 && p0 + r < rows && b * Q8_BLOCK + 4 * c < C) v = *(const uint32_t *)(q + (row0 + r) * C + (size_t)b * Q8_BLOCK + 4 * c);
+    codes[r][c] = v;
+  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const float s = slot >= 0 && p0 + lane < rows ? q8_scale(e[(row0 + lane) * nb + b]) : 0.0f;
+  __syncthreads();
+  if (p0 + lane >= rows) return;
+  typename TT::T *xp = x + ((size_t)img * C + b * Q8_BLOCK) * rows + p0 + lane;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = 32 * w + 4 * j;
+    if (b * Q8_BLOCK + c >= C) break;
+    float f[4];
+    q8_unpack(codes[lane][c / 4], s, f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) xp[(size_t)(c + k) * rows] = TT::put(f[k]);
+  }
+}
+
+// ---------------------------------------------------------------- products
+// out[m][n] = sum over blocks of 2^(ea + eb) * sum of code products, accumulated in fp32 by the matrix cores.  Rows come in
+// segments (rows row_off[s] .. row_off[s + 1] of a, or seg_rows each), a segment is multiplied with the rows of one bank
+// (rows bank_off[g] .. bank_off[g + 1] of b, g = bank_of[s], or s, or 0 where there is one bank): a product of each group of rows with its own matrix, ragged both ways.
+struct Q8Args {
+  const uint8_t *a, *ae, *b, *be;
+  const int32_t *row_off, *bank_off, *bank_of;
+  int seg_rows;       // rows of every segment where row_off is null
+  int n_seg, n_banks;
+  int M, N;           // rows of a, rows of b: what the offsets are clamped to
+  int K, nb;          // channels, blocks of 128
+  int n_cols;         // row length of out
+};
+struct Q8Seg {
+  int r0, r1;         // rows of a
+  int n0, n1;         // rows of b; n0 > n1 never, r0 == r1: nothing to do
+};
+__device__ __forceinline__ void q8_seg_rows(const Q8Args &A, int s, int &r0, int &r1) {
+  if (A.row_off) {
+    r0 = min(max(A.row_off[s], 0), A.M);
+    r1 = max(min(A.row_off[s + 1], A.M), r0);
+  } else {
+    r0 = s * A.seg_rows;
+    r1 = r0 + A.seg_rows;
+  }
+}
+// Tile `work` of all segments' tiles of TM rows in a row: its segment, and the rows it starts at (whole workgroup of 256).
+template <int TM>
+__device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, Q8Seg &S) {
+  __shared__ int found[2], wsum[4];
+  int s, t;
+  if (!A.row_off) {
+    const unsigned per = ((unsigned)A.seg_rows + TM - 1) / TM;
+    s = (int)(work / per);
+    t = (int)(work - (unsigned)s * per);
+    if (s >= A.n_seg) return false;
+  } else {
+    unsigned before = 0;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    s = -1;
+    t = 0;
+    for (int base = 0; base < A.n_seg; base += 256) {
+      const int i = base + (int)threadIdx.x;
+      int tiles = 0;
+      if (i < A.n_seg) {
+        int r0, r1;
+        q8_seg_rows(A, i, r0, r1);
+        tiles = (int)(((unsigned)(r1 - r0) + TM - 1) / TM);
+      }
+      int sum = tiles;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(sum, d);
+        if (lane >= d) sum += o;
+      }
+      if (threadIdx.x == 0) found[0] = -1;
+      if (lane == 63) wsum[w] = sum;
+      __syncthreads();
+      unsigned first = before + (unsigned)(sum - tiles);
+      for (int k = 0; k < w; ++k) first += (unsigned)wsum[k];
+      if (tiles > 0 && work >= first && work - first < (unsigned)tiles) {
+        found[0] = i;
+        found[1] = (int)(work - first);
+      }
+      before += (unsigned)(wsum[0] + wsum[1] + wsum[2] + wsum[3]);
+      __syncthreads();
+      s = found[0];
+      t = found[1];
+      if (s >= 0 || before > work) break;
+      __syncthreads();
+    }
+    if (s < 0) return false;
+  }
+  int r0, r1;
+  q8_seg_rows(A, s, r0, r1);
+  S.r0 = r0 + t * TM;
+  S.r1 = r1;
+  const int g = A.bank_of ? A.bank_of[s] : A.n_banks == 1 ? 0 : s;
+  if (g < 0 || g >= A.n_banks) return false;
+  S.n0 = A.bank_off ? min(max(A.bank_off[g], 0), A.N) : 0;
+  S.n1 = A.bank_off ? max(min(A.bank_off[g + 1], A.N), S.n0) : A.N;
+  return true;
+}
+
+// 32 rows of 64 channels as operands of four v_mfma_f32_32x32x16_bf16.  Lane l holds row l % 32, channels 32 (l / 32) .. + 31, eight for
+// each of the four: which channels meet in which instruction does not matter as long as it is the same for both operands.
+struct Q8Frag { bf8v v[4]; };
+__device__ __forceinline__ bf8v q8_numbers(uint32_t lo, uint32_t hi, float s) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, true);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, true);
+  return bf8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ Q8Frag q8_load(const uint8_t *row, int k, int K, float s) {
+  const u4va z = {0, 0, 0, 0};
+  const u4va lo = k < K ? *(const u4va *)(row + k) : z, hi = k + 16 < K ? *(const u4va *)(row + k + 16) : z;
+  return {{q8_numbers(lo[0], lo[1], s), q8_numbers(lo[2], lo[3], s), q8_numbers(hi[0], hi[1], s), q8_numbers(hi[2], hi[3], s)}};
+}
+__device__ __forceinline__ f16v q8_mfma(const Q8Frag &x, const Q8Frag &y, f16v c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[i], y.v[i], c, 0, 0, 0);
+  return c;
+}
+
+template <class TT>
+__global__ __launch_bounds__(256) void q8_product_kernel(Q8Args A, typename TT::T *__restrict__ out) {
+  Q8Seg S;
+  if (!q8_find<128>(A, blockIdx.x, S)) return;
+  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+  const int cols = min(S.n1 - S.n0, A.n_cols);
+  const int m0 = S.r0 + 32 * (int)(threadIdx.x >> 6), n0 = (int)blockIdx.y * 32;
+  if (m0 >= S.r1 || n0 >= cols) return;
+  const size_t ra = (size_t)min(m0 + i, S.r1 - 1), rb = (size_t)S.n0 + min(n0 + i, cols - 1);
+  f16v acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+  for (int b = 0; b < A.nb; ++b) {
+    const float sa = q8_scale(A.ae[ra * A.nb + b]), sb = q8_scale(A.be[rb * A.nb + b]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int k = b * Q8_BLOCK + 64 * t + 32 * h;
+      acc = q8_mfma(q8_load(A.a + ra * A.K, k, A.K, sa), q8_load(A.b + rb * A.K, k, A.K, sb), acc);
+    }
+  }
+  if (n0 + i >= cols) return;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int m = m0 + 8 * (r >> 2) + 4 * h + (r & 3);
+    if (m < S.r1) out[(size_t)m * A.n_cols + n0 + i] = TT::put(acc[r]);
+  }
+}
+
+// Clutter score: the largest product of a pixel's row with the rows of its bank; NaN where one of them is, -infinity for an empty bank.  The
+// bank is the first operand, so a lane's 16 results are of one pixel and the maximum stays in the lane.
+__global__ __launch_bounds__(256) void q8_score_kernel(Q8Args A, float *__restrict__ out) {
+  Q8Seg S;
+  if (!q8_find<128>(A, blockIdx.x, S)) return;
+  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+  const int m0 = S.r0 + 32 * (int)(threadIdx.x >> 6), rows = S.n1 - S.n0;
+  if (m0 >= S.r1) return;
+  const size_t ra = (size_t)min(m0 + i, S.r1 - 1);
+  float best = -INFINITY;
+  for (int n0 = 0; n0 < rows; n0 += 32) {
+    const size_t rb = (size_t)S.n0 + min(n0 + i, rows - 1);  // rows past the end repeat the last one
+    f16v acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+    for (int b = 0; b < A.nb; ++b) {
+      const float sa = q8_scale(A.ae[ra * A.nb + b]), sb = q8_scale(A.be[rb * A.nb + b]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int k = b * Q8_BLOCK + 64 * t + 32 * h;
+        acc = q8_mfma(q8_load(A.b + rb * A.K, k, A.K, sb), q8_load(A.a + ra * A.K, k, A.K, sa), acc);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) best = __builtin_elementwise_maximum(best, acc[r]);
+  }
+  best = __builtin_elementwise_maximum(best, __shfl_xor(best, 32));
+  if (h == 0 && m0 + i < S.r1) out[m0 + i] = best;
+}
+
+}  // namespace
+#endif  // Q8_KERNELS_HPP

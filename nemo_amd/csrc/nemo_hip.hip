@@ -1245,17 +1245,41 @@ static int q8_operands(nemo_ctx *ctx, const char *who, const uint8_t *d_a, const
   return NEMO_OK;
 }
 
-static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, size_t tiles, int32_t out_dtype, void *d_out, void *stream) {
-  const size_t cols = ((size_t)A.n_cols + 31) / 32;
-  if (tiles > Q8_MAX_BLOCKS || cols > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+}  // extern "C"
+
+// Tiles of tm rows that cover M rows cut into segments, wherever the cuts are (one segment: no more than its own).
+static size_t q8_tiles(const Q8Args &A, size_t tm) {
+  return ((size_t)A.M + tm - 1) / tm + (A.row_off ? (size_t)A.n_seg : 0);
+}
+template <class TT>
+static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, void *d_out, void *stream) {
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
-  const dim3 grid((unsigned)tiles, (unsigned)cols);
-  if (out_dtype == NEMO_F32) hipLaunchKernelGGL((q8_product_kernel<Q8F32>), grid, dim3(256), 0, (hipStream_t)stream, A, (float *)d_out);
-  else hipLaunchKernelGGL((q8_product_kernel<Q8BF16>), grid, dim3(256), 0, (hipStream_t)stream, A, (uint16_t *)d_out);
+  const hipStream_t st = (hipStream_t)stream;
+  typename TT::T *out = (typename TT::T *)d_out;
+  const size_t chunks = ((size_t)A.n_cols + Q8_SR - 1) / Q8_SR, cus = (size_t)ctx->n_cu;
+  // Short rows, and enough of them that 256 a workgroup give half the compute units work with the bank's chunks of 128 dealt out: they stay
+  // in registers and the bank passes by.  A workgroup takes as many chunks as leave 4 workgroups to a compute unit.
+  const size_t tiles = q8_tiles(A, 256);
+  if (A.nb <= 2 && tiles * chunks >= cus / 2 && (size_t)A.M >= 256 * (size_t)A.n_seg) {
+    const int per = (int)std::max<size_t>(1, std::min(chunks, tiles * chunks / (4 * cus)));
+    const size_t cuts = (chunks + per - 1) / per;
+    if (tiles > (1u << 23) - 1 || cuts > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+    const dim3 grid((unsigned)tiles, (unsigned)cuts), wg(512);
+    if (A.nb == 1 && A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, false, 1>), grid, wg, 0, st, A, per, out);
+    else if (A.nb == 1) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, true, 1>), grid, wg, 0, st, A, per, out);
+    else if (A.K == 256) hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, false, 1>), grid, wg, 0, st, A, per, out);
+    else hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, true, 1>), grid, wg, 0, st, A, per, out);
+  } else {
+    const size_t few = q8_tiles(A, 32);
+    if (few > Q8_MAX_BLOCKS || chunks > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+    hipLaunchKernelGGL((q8_product_few_kernel<TT>), dim3((unsigned)few, (unsigned)chunks), dim3(256), 0, st, A, out);
+  }
   HIP_TRY(ctx, hipGetLastError());
   return NEMO_OK;
 }
+
+extern "C" {
 
 int nemo_q8_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be, int32_t N, int32_t K,
                     int32_t out_dtype, void *d_out, void *stream) {
@@ -1268,7 +1292,8 @@ int nemo_q8_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int6
   A.seg_rows = A.M;
   A.n_seg = A.n_banks = 1;
   A.n_cols = N;
-  return q8_launch_product(ctx, "nemo_q8_product", A, ((size_t)M + 127) / 128, out_dtype, d_out, stream);
+  return out_dtype == NEMO_F32 ? q8_launch_product<Q8F32>(ctx, "nemo_q8_product", A, d_out, stream)
+                               : q8_launch_product<Q8BF16>(ctx, "nemo_q8_product", A, d_out, stream);
 }
 
 int nemo_q8_grouped_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const int32_t *d_row_off, int32_t n_seg,
@@ -1287,7 +1312,8 @@ int nemo_q8_grouped_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_
   A.row_off = d_row_off; A.bank_off = d_bank_off; A.bank_of = d_bank_of;
   A.n_seg = n_seg; A.n_banks = n_banks;
   A.n_cols = n_cols;
-  return q8_launch_product(ctx, "nemo_q8_grouped_product", A, ((size_t)M + 127) / 128 + n_seg, out_dtype, d_out, stream);
+  return out_dtype == NEMO_F32 ? q8_launch_product<Q8F32>(ctx, "nemo_q8_grouped_product", A, d_out, stream)
+                               : q8_launch_product<Q8BF16>(ctx, "nemo_q8_grouped_product", A, d_out, stream);
 }
 
 int nemo_q8_clutter_score(nemo_ctx *ctx, const uint8_t *d_feat, const uint8_t *d_feat_e, int32_t n_img, const uint8_t *d_cbank, const uint8_t *d_cbank_e,
@@ -1305,11 +1331,28 @@ int nemo_q8_clutter_score(nemo_ctx *ctx, const uint8_t *d_feat, const uint8_t *d
   A.seg_rows = hw;
   A.n_seg = n_img; A.n_banks = n_banks;
   A.bank_off = d_bank_off; A.bank_of = d_bank_of;
-  const size_t blocks = (size_t)n_img * (((size_t)hw + 127) / 128);
-  if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_q8_clutter_score: too many pixels for one launch");
+  // The largest tile of pixels per workgroup that still gives every compute unit a workgroup; where not even 256 pixels do, 32 with
+  // the bank dealt to the waves.
+  const auto tiles = [&](size_t tm) { return (size_t)n_img * (((size_t)hw + tm - 1) / tm); };
+  const size_t cus = (size_t)ctx->n_cu;
+  const bool wide = ctx->cfg.feat_dim == 256;
+  const int T = !wide && tiles(1024) >= cus ? 4 : tiles(512) >= cus ? 2 : tiles(256) >= cus ? 1 : 0;
+  const size_t blocks = tiles(T ? 256 * T : 32);
+  if (blocks > (1u << 23) - 1) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_q8_clutter_score: too many pixels for one launch");
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
-  hipLaunchKernelGGL(q8_score_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, A, d_out);
+  const dim3 grid((unsigned)blocks), wg(512);
+  const hipStream_t st = (hipStream_t)stream;
+  if (wide) {
+    if (T == 2) hipLaunchKernelGGL((q8_score_kernel<2, 2>), grid, wg, 0, st, A, d_out);
+    else if (T == 1) hipLaunchKernelGGL((q8_score_kernel<2, 1>), grid, wg, 0, st, A, d_out);
+    else hipLaunchKernelGGL((q8_score_few_kernel<2>), grid, wg, 0, st, A, d_out);
+  } else {
+    if (T == 4) hipLaunchKernelGGL((q8_score_kernel<1, 4>), grid, wg, 0, st, A, d_out);
+    else if (T == 2) hipLaunchKernelGGL((q8_score_kernel<1, 2>), grid, wg, 0, st, A, d_out);
+    else if (T == 1) hipLaunchKernelGGL((q8_score_kernel<1, 1>), grid, wg, 0, st, A, d_out);
+    else hipLaunchKernelGGL((q8_score_few_kernel<1>), grid, wg, 0, st, A, d_out);
+  }
   HIP_TRY(ctx, hipGetLastError());
   return NEMO_OK;
 }

@@ -47,12 +47,9 @@ __device__ __forceinline__ void q8_unpack(uint32_t codes, float s, float *x) {
 // the three types a row is quantised from and read back to
 struct Q8F32 { typedef float T; static __device__ __forceinline__ float get(float x) { return x; } static __device__ __forceinline__ float put(float x) { return x; } };
 struct Q8BF16 {
-  typedef uint16_t T;
-  static __device__ __forceinline__ float get(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
-  static __device__ __forceinline__ uint16_t put(float x) {  // nearest even
-    const uint32_t u = __float_as_uint(x);
-    return (u & 0x7fffffffu) > Q8_INF ? (uint16_t)0x7fc0 : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-  }
+  typedef __bf16 T;
+  static __device__ __forceinline__ float get(__bf16 x) { return (float)x; }
+  static __device__ __forceinline__ __bf16 put(float x) { return (__bf16)x; }
 };
 struct Q8F16 {
   typedef _Float16 T;
@@ -289,10 +286,10 @@ __device__ __forceinline__ void q8_seg_rows(const Q8Args &A, int s, int &r0, int
     r1 = r0 + A.seg_rows;
   }
 }
-// Tile `work` of all segments' tiles of TM rows in a row: its segment, and the rows it starts at (whole workgroup of 256).
-template <int TM>
+// Tile `work` of all segments' tiles of TM rows in a row: its segment, and the rows it starts at (whole workgroup).
+template <int TM, int WAVES>
 __device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, Q8Seg &S) {
-  __shared__ int found[2], wsum[4];
+  __shared__ int found[2], wsum[WAVES];
   int s, t;
   if (!A.row_off) {
     const unsigned per = ((unsigned)A.seg_rows + TM - 1) / TM;
@@ -304,7 +301,7 @@ __device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, Q8Seg &S
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     s = -1;
     t = 0;
-    for (int base = 0; base < A.n_seg; base += 256) {
+    for (int base = 0; base < A.n_seg; base += 64 * WAVES) {
       const int i = base + (int)threadIdx.x;
       int tiles = 0;
       if (i < A.n_seg) {
@@ -327,10 +324,11 @@ __device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, Q8Seg &S
         found[0] = i;
         found[1] = (int)(work - first);
       }
-      before += (unsigned)(wsum[0] + wsum[1] + wsum[2] + wsum[3]);
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) before += (unsigned)wsum[k];
       __syncthreads();
-      s = found[0];
-      t = found[1];
+      s = __builtin_amdgcn_readfirstlane(found[0]);
+      t = __builtin_amdgcn_readfirstlane(found[1]);
       if (s >= 0 || before > work) break;
       __syncthreads();
     }
@@ -347,81 +345,290 @@ __device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, Q8Seg &S
   return true;
 }
 
-// 32 rows of 64 channels as operands of four v_mfma_f32_32x32x16_bf16.  Lane l holds row l % 32, channels 32 (l / 32) .. + 31, eight for
-// each of the four: which channels meet in which instruction does not matter as long as it is the same for both operands.
-struct Q8Frag { bf8v v[4]; };
+// Operands of v_mfma_f32_32x32x16_bf16: lane l holds row l % 32 and, of a block of 128 channels, the 16-byte chunks 2 u + l / 32, u = 0 .. 3.
+// A chunk feeds two instructions, eight channels each; which channels meet in which instruction does not matter as long as it is the
+// same for both operands (and it is the same in every kernel here, so a product has the same bits whichever computes it).
 __device__ __forceinline__ bf8v q8_numbers(uint32_t lo, uint32_t hi, float s) {
   const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, true);
   const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, true);
   return bf8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-__device__ __forceinline__ Q8Frag q8_load(const uint8_t *row, int k, int K, float s) {
-  const u4va z = {0, 0, 0, 0};
-  const u4va lo = k < K ? *(const u4va *)(row + k) : z, hi = k + 16 < K ? *(const u4va *)(row + k + 16) : z;
-  return {{q8_numbers(lo[0], lo[1], s), q8_numbers(lo[2], lo[3], s), q8_numbers(hi[0], hi[1], s), q8_numbers(hi[2], hi[3], s)}};
+// The wave's 64 lanes copy 16 bytes each from their own address to consecutive places of LDS, without going through registers; complete
+// after q8_wait_copies() and a barrier.
+__device__ __forceinline__ void q8_copy16(const uint8_t *from, uint8_t *lds) {
+  __builtin_amdgcn_global_load_lds((const uint32_t GAS *)(uintptr_t)from, (__attribute__((address_space(3))) uint32_t *)lds, 16, 0, 0);
+}
+__device__ __forceinline__ void q8_wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+struct Q8Frag { bf8v v[8]; };  // 32 rows of 128 channels
+struct Q8Raw { u4va v[4]; };   // the same as codes
+__device__ __forceinline__ Q8Raw q8_load(const uint8_t *row, int b, int h, int K) {
+  Q8Raw x;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int k = b * Q8_BLOCK + 16 * (2 * u + h);
+    x.v[u] = k < K ? *(const u4va *)(row + k) : u4va{0, 0, 0, 0};
+  }
+  return x;
+}
+__device__ __forceinline__ Q8Frag q8_frag(const Q8Raw &x, float s) {
+  Q8Frag f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    f.v[2 * u] = q8_numbers(x.v[u][0], x.v[u][1], s);
+    f.v[2 * u + 1] = q8_numbers(x.v[u][2], x.v[u][3], s);
+  }
+  return f;
 }
 __device__ __forceinline__ f16v q8_mfma(const Q8Frag &x, const Q8Frag &y, f16v c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[i], y.v[i], c, 0, 0, 0);
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[i], y.v[i], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f16v q8_zero() {
+  f16v c;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) c[r] = 0.0f;
   return c;
 }
 
+// Stores one 32 x 32 tile of products: lane l has column l % 32 of rows 8 (r / 4) + 4 (l / 32) + r % 4.  m0, m1, n0 and n1 are the same
+// for the whole wave: a row's address is a scalar, a lane's place in it 32 bits.
 template <class TT>
-__global__ __launch_bounds__(256) void q8_product_kernel(Q8Args A, typename TT::T *__restrict__ out) {
-  Q8Seg S;
-  if (!q8_find<128>(A, blockIdx.x, S)) return;
-  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
-  const int cols = min(S.n1 - S.n0, A.n_cols);
-  const int m0 = S.r0 + 32 * (int)(threadIdx.x >> 6), n0 = (int)blockIdx.y * 32;
-  if (m0 >= S.r1 || n0 >= cols) return;
-  const size_t ra = (size_t)min(m0 + i, S.r1 - 1), rb = (size_t)S.n0 + min(n0 + i, cols - 1);
-  f16v acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-  for (int b = 0; b < A.nb; ++b) {
-    const float sa = q8_scale(A.ae[ra * A.nb + b]), sb = q8_scale(A.be[rb * A.nb + b]);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int k = b * Q8_BLOCK + 64 * t + 32 * h;
-      acc = q8_mfma(q8_load(A.a + ra * A.K, k, A.K, sa), q8_load(A.b + rb * A.K, k, A.K, sb), acc);
-    }
-  }
-  if (n0 + i >= cols) return;
+__device__ __forceinline__ void q8_store(typename TT::T *out, int ld, int m0, int m1, int n0, int n1, int i, int h, const f16v &acc) {
+  typedef typename TT::T T;
+  if (n0 + i >= n1) return;
+  const uint32_t at = (uint32_t)(4 * h * ld + i) * (uint32_t)sizeof(T);
+  char *base = (char *)(out + (size_t)m0 * ld + n0);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int m = m0 + 8 * (r >> 2) + 4 * h + (r & 3);
-    if (m < S.r1) out[(size_t)m * A.n_cols + n0 + i] = TT::put(acc[r]);
+    const int row = 8 * (r >> 2) + (r & 3);
+    T GAS *p = (T GAS *)(uintptr_t)(base + (size_t)row * ld * sizeof(T) + at);
+    if (m0 + 32 <= m1 || m0 + row + 4 * h < m1) *p = TT::put(acc[r]);
   }
 }
 
-// Clutter score: the largest product of a pixel's row with the rows of its bank; NaN where one of them is, -infinity for an empty bank.  The
-// bank is the first operand, so a lane's 16 results are of one pixel and the maximum stays in the lane.
-__global__ __launch_bounds__(256) void q8_score_kernel(Q8Args A, float *__restrict__ out) {
+// Few rows: a wave owns 32 rows x 32 columns, a workgroup 4 such tiles side by side; operands come straight from memory, a block of 128
+// channels ahead.  Any K.
+template <class TT>
+__global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, typename TT::T *__restrict__ out) {
   Q8Seg S;
-  if (!q8_find<128>(A, blockIdx.x, S)) return;
+  if (!q8_find<32, 4>(A, blockIdx.x, S)) return;
   const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
-  const int m0 = S.r0 + 32 * (int)(threadIdx.x >> 6), rows = S.n1 - S.n0;
-  if (m0 >= S.r1) return;
-  const size_t ra = (size_t)min(m0 + i, S.r1 - 1);
-  float best = -INFINITY;
-  for (int n0 = 0; n0 < rows; n0 += 32) {
-    const size_t rb = (size_t)S.n0 + min(n0 + i, rows - 1);  // rows past the end repeat the last one
-    f16v acc;
+  const int cols = min(S.n1 - S.n0, A.n_cols);
+  const int n0 = ((int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)) * 32;
+  if (n0 >= cols) return;
+  const size_t ra = (size_t)min(S.r0 + i, S.r1 - 1), rb = (size_t)S.n0 + min(n0 + i, cols - 1);
+  f16v acc = q8_zero();
+  Q8Raw xa = q8_load(A.a + ra * A.K, 0, h, A.K), xb = q8_load(A.b + rb * A.K, 0, h, A.K);
+  uint32_t ea = A.ae[ra * A.nb], eb = A.be[rb * A.nb];
+  for (int b = 0; b < A.nb; ++b) {
+    const Q8Frag fa = q8_frag(xa, q8_scale(ea)), fb = q8_frag(xb, q8_scale(eb));
+    if (b + 1 < A.nb) {
+      xa = q8_load(A.a + ra * A.K, b + 1, h, A.K);
+      xb = q8_load(A.b + rb * A.K, b + 1, h, A.K);
+      ea = A.ae[ra * A.nb + b + 1];
+      eb = A.be[rb * A.nb + b + 1];
+    }
+    acc = q8_mfma(fa, fb, acc);
+  }
+  q8_store<TT>(out, A.n_cols, S.r0, S.r1, n0, cols, i, h, acc);
+}
+
+// The bank's way to LDS, for the kernels that keep their rows of a in registers (8 waves, K <= 128 NB).  The bank goes through LDS as
+// codes, 128 rows at a time, copied there by the memory unit while the chunk before is multiplied (two buffers, one barrier a
+// chunk).  A row is 8 NB chunks of 16 bytes, chunk c at place c ^ (row & 7): the copy fills places in order of lanes, and the 8
+// rows that a read of one chunk touches lie in different banks of the LDS.
+constexpr int Q8_SR = 128;  // bank rows per buffer
+template <int NB, bool TAIL>  // TAIL: K is less than 128 NB
+struct Q8Bank {
+  static constexpr int RB = Q8_BLOCK * NB;                  // bytes of a row in LDS
+  static constexpr int PER = Q8_SR * RB / (512 * 16);       // 16-byte copies per thread and buffer
+  uint8_t codes[2][Q8_SR * RB];
+  float scale[2][Q8_SR * NB];
+  // starts copying rows 128 c .. of the bank's `rows`; returns the scale byte that put_scale takes once it is needed
+  __device__ __forceinline__ uint32_t copy(const uint8_t *bank, const uint8_t *bank_e, int K, int rows, int c, int tid) {
+    const int lane = tid & 63, w = tid >> 6;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-    for (int b = 0; b < A.nb; ++b) {
-      const float sa = q8_scale(A.ae[ra * A.nb + b]), sb = q8_scale(A.be[rb * A.nb + b]);
+    for (int j = 0; j < PER; ++j) {
+      const int place = (w * PER + j) * 64 + lane, r = place / (8 * NB), q = (place % (8 * NB)) ^ (r & 7);
+      const int row = min(c * Q8_SR + r, rows - 1);         // rows past the end repeat the last one
+      q8_copy16(bank + (TAIL ? (size_t)row * K + min(16 * q, K - 16) : (size_t)row * RB + 16 * q), &codes[c & 1][(w * PER + j) * 1024]);
+    }
+    return tid < Q8_SR * NB ? bank_e[(size_t)min(c * Q8_SR + tid / NB, rows - 1) * NB + tid % NB] : 0;
+  }
+  __device__ __forceinline__ void put_scale(int c, int tid, uint32_t e) {
+    if (tid < Q8_SR * NB) scale[c & 1][tid] = q8_scale(e);
+  }
+  // rows n .. n + 31 of buffer c & 1
+  __device__ __forceinline__ void get(int c, int n, int i, int h, int K, Q8Frag (&y)[NB]) const {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int k = b * Q8_BLOCK + 64 * t + 32 * h;
-        acc = q8_mfma(q8_load(A.b + rb * A.K, k, A.K, sb), q8_load(A.a + ra * A.K, k, A.K, sa), acc);
+    for (int b = 0; b < NB; ++b) {
+      Q8Raw raw;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int q = 8 * b + 2 * u + h;
+        raw.v[u] = *(const u4va *)&codes[c & 1][(n + i) * RB + 16 * (q ^ (i & 7))];
+        if (TAIL && 16 * q >= K) raw.v[u] = u4va{0, 0, 0, 0};
+      }
+      y[b] = q8_frag(raw, scale[c & 1][(n + i) * NB + b]);
+    }
+  }
+};
+
+// Short rows (K <= 256), many of them: 8 waves keep T x 32 rows of a each in registers and multiply them with the bank's rows of chunks
+// blockIdx.y * per .. + per.
+template <class TT, int NB, bool TAIL, int T>
+__global__ __launch_bounds__(512, T * NB > 2 ? 2 : 4) void q8_product_short_kernel(Q8Args A, int per, typename TT::T *__restrict__ out) {
+  __shared__ __align__(16) Q8Bank<NB, TAIL> L;
+  Q8Seg S;
+  if (!q8_find<256 * T, 8>(A, blockIdx.x, S)) return;
+  const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cols = min(S.n1 - S.n0, A.n_cols), m0 = S.r0 + 32 * T * w;
+  const int first = (int)blockIdx.y * per, chunks = min((cols + Q8_SR - 1) / Q8_SR, first + per);
+  if (first >= chunks) return;
+  const uint8_t *bank = A.b + (size_t)S.n0 * A.K, *bank_e = A.be + (size_t)S.n0 * NB;
+  uint32_t e = L.copy(bank, bank_e, A.K, cols, first, tid);
+  Q8Frag x[T][NB];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const size_t row = (size_t)min(m0 + 32 * t + i, S.r1 - 1);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) x[t][b] = q8_frag(q8_load(A.a + row * A.K, b, h, A.K), q8_scale(A.ae[row * NB + b]));
+  }
+  L.put_scale(first, tid, e);
+  q8_wait_copies();
+  __syncthreads();
+  for (int c = first; c < chunks; ++c) {
+    if (c + 1 < chunks) e = L.copy(bank, bank_e, A.K, cols, c + 1, tid);
+    const int left = min(cols - c * Q8_SR, Q8_SR);
+    for (int n = 0; n < left; n += 32) {
+      Q8Frag y[NB];
+      L.get(c, n, i, h, A.K, y);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        if (m0 + 32 * t >= S.r1) break;
+        f16v acc = q8_zero();
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc = q8_mfma(x[t][b], y[b], acc);
+        q8_store<TT>(out, A.n_cols, m0 + 32 * t, S.r1, c * Q8_SR + n, cols, i, h, acc);
       }
     }
+    if (c + 1 < chunks) L.put_scale(c + 1, tid, e);
+    q8_wait_copies();
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- clutter score
+// The largest product of a pixel's row with the rows of its image's bank; NaN where one of them is, -infinity for an empty bank.  The
+// bank is the first operand, so a lane's 16 results are of one pixel and the maximum stays in the lane: 8 three-way
+// maxima (v_maximum3_f32, which keeps NaN) per 8 NB matrix instructions.
+__device__ __forceinline__ float q8_max(float best, const f16v &acc) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) best = __builtin_elementwise_maximum(best, acc[r]);
+  for (int r = 0; r < 16; ++r) best = __builtin_elementwise_maximum(best, acc[r]);
+  return best;
+}
+// 8 waves, each with the numbers of T x 32 pixels in registers: a row tile of the bank is read and widened once per wave and meets T
+// tiles of pixels.
+template <int NB, int T>
+__global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Args A, float *__restrict__ out) {
+  constexpr int K = Q8_BLOCK * NB;
+  __shared__ __align__(16) Q8Bank<NB, false> L;
+  Q8Seg S;
+  if (!q8_find<256 * T, 8>(A, blockIdx.x, S)) return;
+  const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = tid >> 6;
+  const int rows = S.n1 - S.n0, m0 = S.r0 + 32 * T * w;
+  const uint8_t *bank = A.b + (size_t)S.n0 * K, *bank_e = A.be + (size_t)S.n0 * NB;
+  float best[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) best[t] = -INFINITY;
+  if (rows > 0) {
+    uint32_t e = L.copy(bank, bank_e, K, rows, 0, tid);
+    Q8Frag x[T][NB];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const size_t row = (size_t)min(m0 + 32 * t + i, S.r1 - 1);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) x[t][b] = q8_frag(q8_load(A.a + row * K, b, h, K), q8_scale(A.ae[row * NB + b]));
+    }
+    L.put_scale(0, tid, e);
+    q8_wait_copies();
+    __syncthreads();
+    const int chunks = (rows + Q8_SR - 1) / Q8_SR;
+    for (int c = 0; c < chunks; ++c) {
+      if (c + 1 < chunks) e = L.copy(bank, bank_e, K, rows, c + 1, tid);
+      if (m0 < S.r1) {
+        const int left = min(rows - c * Q8_SR, Q8_SR);
+        for (int n = 0; n < left; n += 32) {
+          Q8Frag y[NB];
+          L.get(c, n, i, h, K, y);
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            f16v acc = q8_zero();
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc = q8_mfma(y[b], x[t][b], acc);
+            best[t] = q8_max(best[t], acc);
+          }
+        }
+      }
+      if (c + 1 < chunks) L.put_scale(c + 1, tid, e);
+      q8_wait_copies();
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const float top = __builtin_elementwise_maximum(best[t], __shfl_xor(best[t], 32));
+    const int m = m0 + 32 * t + i;
+    if (h == 0 && m < S.r1) out[m] = top;
+  }
+}
+// Few pixels: the 8 waves share 32 pixels and deal the bank's row tiles among them; the bank comes straight from memory, a tile ahead.
+template <int NB>
+__global__ __launch_bounds__(512) void q8_score_few_kernel(Q8Args A, float *__restrict__ out) {
+  constexpr int RB = Q8_BLOCK * NB;
+  __shared__ float top[8][32];
+  Q8Seg S;
+  if (!q8_find<32, 8>(A, blockIdx.x, S)) return;
+  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, w = threadIdx.x >> 6;
+  const int rows = S.n1 - S.n0;
+  float best = -INFINITY;
+  if (32 * w < rows) {
+    const size_t row = (size_t)min(S.r0 + i, S.r1 - 1);
+    Q8Raw raw[NB];
+    uint32_t e[NB];
+    auto fetch = [&](int n) {
+      const size_t rb = (size_t)S.n0 + min(n + i, rows - 1);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        raw[b] = q8_load(A.b + rb * RB, b, h, RB);
+        e[b] = A.be[rb * NB + b];
+      }
+    };
+    fetch(32 * w);
+    Q8Frag x[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) x[b] = q8_frag(q8_load(A.a + row * RB, b, h, RB), q8_scale(A.ae[row * NB + b]));
+    for (int n = 32 * w; n < rows; n += 256) {
+      Q8Frag y[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) y[b] = q8_frag(raw[b], q8_scale(e[b]));
+      if (n + 256 < rows) fetch(n + 256);
+      f16v acc = q8_zero();
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc = q8_mfma(y[b], x[b], acc);
+      best = q8_max(best, acc);
+    }
   }
   best = __builtin_elementwise_maximum(best, __shfl_xor(best, 32));
-  if (h == 0 && m0 + i < S.r1) out[m0 + i] = best;
+  if (h == 0) top[w][i] = best;
+  __syncthreads();
+  if (threadIdx.x < 32 && S.r0 + (int)threadIdx.x < S.r1) {
+    float m = top[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = __builtin_elementwise_maximum(m, top[k][threadIdx.x]);
+    out[S.r0 + threadIdx.x] = m;
+  }
 }
 
 }  // namespace

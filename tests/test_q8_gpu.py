@@ -139,7 +139,8 @@ def test_offsets_beyond_32_bits(eng):
 # ------------------------------------------------------------------------------------------------ products
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('m,n,k', [(1, 1, 16), (1, 1088, 128), (33, 31, 128), (127, 129, 144), (128, 128, 256), (200, 1, 512), (257, 300, 240),
-                                   (1000, 77, 128), (129, 260, 2048), (64, 33, 4112)])
+                                   (1000, 77, 128), (129, 260, 2048), (64, 33, 4112),
+                                   (8000, 1088, 128), (33001, 77, 256), (17000, 261, 64), (9001, 1000, 240)])
 def test_product(eng, m, n, k, dtype):
     (a, a64), (b, b64) = rows8(m, k, m + k), rows8(n, k, n + k + 1)
     got = eng.q8_product(a, b, dtype=dtype)
@@ -188,6 +189,9 @@ def offsets(sizes):
     ([64, 64, 200], [130], None, 256),
     ([31, 129, 7, 100], [50, 160, 20], [2, 0, 5, 0], 144),
     ([300, 2, 0, 5], [10, 1], [1, 0, 1, -1], 512),
+    ([5000, 300, 20000, 7, 0, 8000], [300, 500, 129, 1000, 3, 1], None, 128),
+    ([9000, 8500, 300], [1, 515], [1, 1, 0], 256),
+    ([12000, 5000], [130, 700], None, 80),
     ([(i * 37) % 90 for i in range(700)], [(i * 13) % 41 for i in range(700)], None, 128),
 ])
 def test_grouped_product(eng, sizes, banks, bank_of, k, dtype):
@@ -230,7 +234,8 @@ def score64(a64, b64):
 
 
 @pytest.mark.parametrize('d', [128, 256])
-@pytest.mark.parametrize('n,h,w,banks', [(1, 12, 23, [1]), (3, 5, 7, [64]), (5, 8, 16, [33, 0, 1, 200]), (2, 1, 1, [2560]), (7, 9, 31, [5, 17, 31, 32, 96, 513])])
+@pytest.mark.parametrize('n,h,w,banks', [(1, 12, 23, [1]), (3, 5, 7, [64]), (5, 8, 16, [33, 0, 1, 200]), (2, 1, 1, [2560]), (7, 9, 31, [5, 17, 31, 32, 96, 513]),
+                                         (260, 5, 7, [33, 0, 1, 200, 130]), (130, 24, 30, [129, 40]), (130, 15, 20, [300, 1, 31])])
 def test_clutter_score(n, h, w, banks, d):
     from nemo_amd.engine import PoseEngine
     eng = PoseEngine(max(h, w, 24), (h, w), d)
@@ -238,7 +243,7 @@ def test_clutter_score(n, h, w, banks, d):
     a = q8.Q8(a.codes.view(n, h, w, d), a.scale.view(n, h, w, d // 128))
     a64 = a64.view(n, h * w, d)
     of = [(3 * i + 1) % len(banks) for i in range(n)]
-    starts = np.cumsum([0] + banks)
+    starts = np.cumsum([0] + banks)   # (the last three: enough tiles of 1024, 512 and 256 pixels to fill the GPU with them)
     out = torch.full((n, h, w), 5.0, device='cuda')
     index = torch.tensor(of, dtype=torch.int32)
     if n > 2:

@@ -1257,19 +1257,25 @@ static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, vo
   HIP_TRY(ctx, on.status);
   const hipStream_t st = (hipStream_t)stream;
   typename TT::T *out = (typename TT::T *)d_out;
-  const size_t chunks = ((size_t)A.n_cols + Q8_SR - 1) / Q8_SR, cus = (size_t)ctx->n_cu;
-  // Short rows, and enough of them that 256 a workgroup give half the compute units work with the bank's chunks of 128 dealt out: they stay
-  // in registers and the bank passes by.  A workgroup takes as many chunks as leave 4 workgroups to a compute unit.
-  const size_t tiles = q8_tiles(A, 256);
-  if (A.nb <= 2 && tiles * chunks >= cus / 2 && (size_t)A.M >= 256 * (size_t)A.n_seg) {
-    const int per = (int)std::max<size_t>(1, std::min(chunks, tiles * chunks / (4 * cus)));
-    const size_t cuts = (chunks + per - 1) / per;
-    if (tiles > (1u << 23) - 1 || cuts > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
-    const dim3 grid((unsigned)tiles, (unsigned)cuts), wg(512);
-    if (A.nb == 1 && A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, false, 1>), grid, wg, 0, st, A, per, out);
-    else if (A.nb == 1) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, true, 1>), grid, wg, 0, st, A, per, out);
-    else if (A.K == 256) hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, false, 1>), grid, wg, 0, st, A, per, out);
-    else hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, true, 1>), grid, wg, 0, st, A, per, out);
+  const size_t chunks = ((size_t)A.n_cols + 127) / 128, cus = (size_t)ctx->n_cu;
+  // Short rows: 8 waves over 512 / nb columns, or 8 / wc of them to the same columns where there are fewer.  As many rows to a workgroup, up to
+  // 128 (f32) or 256 (bf16: the same bytes of results), as still give 2 workgroups to a compute unit.
+  const int per_wave = A.nb == 1 ? 64 : 32;
+  int wc = 8;
+  while (wc > 1 && A.n_cols <= per_wave * (wc / 2)) wc /= 2;
+  const size_t cuts = ((size_t)A.n_cols + per_wave * wc - 1) / ((size_t)per_wave * wc);
+  int rt = (sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR) / 32;
+  while (rt > 8 / wc && rt > 1 && q8_tiles(A, 32 * rt) * cuts < 2 * cus) rt /= 2;
+  const size_t tiles = q8_tiles(A, 32 * rt);
+  if (A.nb <= 2 && (size_t)A.M >= 64 * (size_t)A.n_seg && tiles * cuts >= cus / 4) {
+    const size_t blocks = (tiles * cuts + 7) / 8 * 8;
+    if (blocks > (1u << 23) - 1) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+    const dim3 grid((unsigned)blocks), wg(512);
+    const int n = (int)tiles, c = (int)cuts;
+    if (A.nb == 1 && A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, false>), grid, wg, 0, st, A, n, c, wc, rt, out);
+    else if (A.nb == 1) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, true>), grid, wg, 0, st, A, n, c, wc, rt, out);
+    else if (A.K == 256) hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, false>), grid, wg, 0, st, A, n, c, wc, rt, out);
+    else hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, true>), grid, wg, 0, st, A, n, c, wc, rt, out);
   } else {
     const size_t few = q8_tiles(A, 32);
     if (few > Q8_MAX_BLOCKS || chunks > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);

@@ -287,8 +287,8 @@ __device__ __forceinline__ void q8_seg_rows(const Q8Args &A, int s, int &r0, int
   }
 }
 // Tile `work` of all segments' tiles of TM rows in a row: its segment, and the rows it starts at (whole workgroup).
-template <int TM, int WAVES>
-__device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, Q8Seg &S) {
+template <int WAVES>
+__device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, int TM, Q8Seg &S) {
   __shared__ int found[2], wsum[WAVES];
   int s, t;
   if (!A.row_off) {
@@ -358,7 +358,13 @@ __device__ __forceinline__ bf8v q8_numbers(uint32_t lo, uint32_t hi, float s) {
 __device__ __forceinline__ void q8_copy16(const uint8_t *from, uint8_t *lds) {
   __builtin_amdgcn_global_load_lds((const uint32_t GAS *)(uintptr_t)from, (__attribute__((address_space(3))) uint32_t *)lds, 16, 0, 0);
 }
-__device__ __forceinline__ void q8_wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void q8_wait_copies() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+// What the wave's lanes wrote to LDS before, its lanes read after.
+__device__ __forceinline__ void q8_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 struct Q8Frag { bf8v v[8]; };  // 32 rows of 128 channels
 struct Q8Raw { u4va v[4]; };   // the same as codes
 __device__ __forceinline__ Q8Raw q8_load(const uint8_t *row, int b, int h, int K) {
@@ -399,11 +405,14 @@ __device__ __forceinline__ void q8_store(typename TT::T *out, int ld, int m0, in
   if (n0 + i >= n1) return;
   const uint32_t at = (uint32_t)(4 * h * ld + i) * (uint32_t)sizeof(T);
   char *base = (char *)(out + (size_t)m0 * ld + n0);
+  auto to = [&](int r) { return (T GAS *)(uintptr_t)(base + (size_t)(8 * (r >> 2) + (r & 3)) * ld * sizeof(T) + at); };
+  if (m0 + 32 <= m1) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int row = 8 * (r >> 2) + (r & 3);
-    T GAS *p = (T GAS *)(uintptr_t)(base + (size_t)row * ld * sizeof(T) + at);
-    if (m0 + 32 <= m1 || m0 + row + 4 * h < m1) *p = TT::put(acc[r]);
+    for (int r = 0; r < 16; ++r) *to(r) = TT::put(acc[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (m0 + 8 * (r >> 2) + (r & 3) + 4 * h < m1) *to(r) = TT::put(acc[r]);
   }
 }
 
@@ -412,7 +421,7 @@ __device__ __forceinline__ void q8_store(typename TT::T *out, int ld, int m0, in
 template <class TT>
 __global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, typename TT::T *__restrict__ out) {
   Q8Seg S;
-  if (!q8_find<32, 4>(A, blockIdx.x, S)) return;
+  if (!q8_find<4>(A, blockIdx.x, 32, S)) return;
   const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
   const int cols = min(S.n1 - S.n0, A.n_cols);
   const int n0 = ((int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)) * 32;
@@ -434,88 +443,156 @@ __global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, typename 
   q8_store<TT>(out, A.n_cols, S.r0, S.r1, n0, cols, i, h, acc);
 }
 
-// The bank's way to LDS, for the kernels that keep their rows of a in registers (8 waves, K <= 128 NB).  The bank goes through LDS as
-// codes, 128 rows at a time, copied there by the memory unit while the chunk before is multiplied (two buffers, one barrier a
-// chunk).  A row is 8 NB chunks of 16 bytes, chunk c at place c ^ (row & 7): the copy fills places in order of lanes, and the 8
-// rows that a read of one chunk touches lie in different banks of the LDS.
-constexpr int Q8_SR = 128;  // bank rows per buffer
-template <int NB, bool TAIL>  // TAIL: K is less than 128 NB
+// The bank's way to LDS, for the kernels that keep their rows of a in registers (8 waves, K <= 128 NB): SR rows at a time as codes, copied
+// by the memory unit.  A row is 8 NB chunks of 16 bytes, chunk c at place c ^ (row / NT & 7): the copy fills places in order of
+// lanes, and the 8 rows (NT apart) that a read of one chunk touches lie in different banks of the LDS.
+template <int NB, bool TAIL, int SR, int BUFS, int NT>  // TAIL: K is less than 128 NB; NT: rows that a lane reads side by side
 struct Q8Bank {
   static constexpr int RB = Q8_BLOCK * NB;                  // bytes of a row in LDS
-  static constexpr int PER = Q8_SR * RB / (512 * 16);       // 16-byte copies per thread and buffer
-  uint8_t codes[2][Q8_SR * RB];
-  float scale[2][Q8_SR * NB];
-  // starts copying rows 128 c .. of the bank's `rows`; returns the scale byte that put_scale takes once it is needed
-  __device__ __forceinline__ uint32_t copy(const uint8_t *bank, const uint8_t *bank_e, int K, int rows, int c, int tid) {
+  static constexpr int PER = SR * RB / (512 * 16);          // 16-byte copies per thread and buffer
+  static constexpr int NE = (SR * NB + 511) / 512;          // scales per thread and buffer
+  static_assert(PER * 512 * 16 == SR * RB && SR % 32 == 0, "");
+  uint8_t codes[BUFS][SR * RB];
+  float scale[BUFS][SR * NB];
+  // starts copying `room` rows (whole 8 KB) from row `first` of the bank's `rows` on; the scale bytes stay in e until put_scale
+  __device__ __forceinline__ void copy(int buf, const uint8_t *bank, const uint8_t *bank_e, int K, int rows, int first, int room, int tid, uint32_t (&e)[NE]) {
     const int lane = tid & 63, w = tid >> 6;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int place = (w * PER + j) * 64 + lane, r = place / (8 * NB), q = (place % (8 * NB)) ^ (r & 7);
-      const int row = min(c * Q8_SR + r, rows - 1);         // rows past the end repeat the last one
-      q8_copy16(bank + (TAIL ? (size_t)row * K + min(16 * q, K - 16) : (size_t)row * RB + 16 * q), &codes[c & 1][(w * PER + j) * 1024]);
+      if (8192 * j >= room * RB) break;
+      const int place = (8 * j + w) * 64 + lane, r = place / (8 * NB), q = (place % (8 * NB)) ^ (r / NT & 7);
+      const int row = min(first + r, rows - 1);             // rows past the end repeat the last one
+      q8_copy16(bank + (TAIL ? (size_t)row * K + min(16 * q, K - 16) : (size_t)row * RB + 16 * q), &codes[buf][(8 * j + w) * 1024]);
     }
-    return tid < Q8_SR * NB ? bank_e[(size_t)min(c * Q8_SR + tid / NB, rows - 1) * NB + tid % NB] : 0;
-  }
-  __device__ __forceinline__ void put_scale(int c, int tid, uint32_t e) {
-    if (tid < Q8_SR * NB) scale[c & 1][tid] = q8_scale(e);
-  }
-  // rows n .. n + 31 of buffer c & 1
-  __device__ __forceinline__ void get(int c, int n, int i, int h, int K, Q8Frag (&y)[NB]) const {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      Q8Raw raw;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int q = 8 * b + 2 * u + h;
-        raw.v[u] = *(const u4va *)&codes[c & 1][(n + i) * RB + 16 * (q ^ (i & 7))];
-        if (TAIL && 16 * q >= K) raw.v[u] = u4va{0, 0, 0, 0};
-      }
-      y[b] = q8_frag(raw, scale[c & 1][(n + i) * NB + b]);
+    for (int j = 0; j < NE; ++j) {
+      const int k = tid + 512 * j;
+      e[j] = k < SR * NB ? bank_e[(size_t)min(first + k / NB, rows - 1) * NB + k % NB] : 0;
     }
+  }
+  __device__ __forceinline__ void put_scale(int buf, int tid, const uint32_t (&e)[NE]) {
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+      if (tid + 512 * j < SR * NB) scale[buf][tid + 512 * j] = q8_scale(e[j]);
+  }
+  // rows n + NT i, i = 0 .. 31, of a buffer
+  __device__ __forceinline__ Q8Frag get(int buf, int n, int b, int i, int h, int K) const {
+    Q8Raw raw;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int q = 8 * b + 2 * u + h;
+      raw.v[u] = *(const u4va *)&codes[buf][(n + NT * i) * RB + 16 * (q ^ (i & 7))];
+      if (TAIL && 16 * q >= K) raw.v[u] = u4va{0, 0, 0, 0};
+    }
+    return q8_frag(raw, scale[buf][(n + NT * i) * NB + b]);
   }
 };
 
-// Short rows (K <= 256), many of them: 8 waves keep T x 32 rows of a each in registers and multiply them with the bank's rows of chunks
-// blockIdx.y * per .. + per.
-template <class TT, int NB, bool TAIL, int T>
-__global__ __launch_bounds__(512, T * NB > 2 ? 2 : 4) void q8_product_short_kernel(Q8Args A, int per, typename TT::T *__restrict__ out) {
-  __shared__ __align__(16) Q8Bank<NB, TAIL> L;
-  Q8Seg S;
-  if (!q8_find<256 * T, 8>(A, blockIdx.x, S)) return;
-  const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cols = min(S.n1 - S.n0, A.n_cols), m0 = S.r0 + 32 * T * w;
-  const int first = (int)blockIdx.y * per, chunks = min((cols + Q8_SR - 1) / Q8_SR, first + per);
-  if (first >= chunks) return;
-  const uint8_t *bank = A.b + (size_t)S.n0 * A.K, *bank_e = A.be + (size_t)S.n0 * NB;
-  uint32_t e = L.copy(bank, bank_e, A.K, cols, first, tid);
-  Q8Frag x[T][NB];
+// Products leave in groups of NT tiles of 32 columns, tile t with columns NT i + t, so that a lane has NT neighbouring ones: 16 stores
+// of 8 bytes a lane and whole lines a row, at any alignment of out's rows (the bf16 result's rows of an odd length begin in
+// the middle of a word).
+template <class TT, int NT> struct __attribute__((packed, aligned(sizeof(typename TT::T)))) Q8Out { typename TT::T v[NT]; };
+template <class TT, int NT>
+__device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int m0, int m1, int n0, int n1, int i, int h, const f16v (&acc)[NT]) {
+  typedef typename TT::T T;
+  const uint32_t at = (uint32_t)(4 * h * ld + NT * i) * (uint32_t)sizeof(T);
+  char *base = (char *)(out + (size_t)m0 * ld + n0);
+  auto to = [&](int r) { return base + (size_t)(8 * (r >> 2) + (r & 3)) * ld * sizeof(T) + at; };
+  if (m0 + 32 <= m1 && n0 + 32 * NT <= n1) {
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const size_t row = (size_t)min(m0 + 32 * t + i, S.r1 - 1);
+    for (int r = 0; r < 16; ++r) {
+      Q8Out<TT, NT> o;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) x[t][b] = q8_frag(q8_load(A.a + row * A.K, b, h, A.K), q8_scale(A.ae[row * NB + b]));
+      for (int t = 0; t < NT; ++t) o.v[t] = TT::put(acc[t][r]);
+      *(Q8Out<TT, NT> *)to(r) = o;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (n0 + NT * i + t >= n1) break;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (m0 + 8 * (r >> 2) + (r & 3) + 4 * h < m1) ((T *)to(r))[t] = TT::put(acc[t][r]);
+    }
   }
-  L.put_scale(first, tid, e);
+}
+// Short rows (K <= 256).  What bounds these products is the result's way to memory (a row of 128 channels meets a row of the bank in 256
+// operations, but leaves 4 bytes), so the work is cut for the stores: the 8 waves of a workgroup own neighbouring columns of the same
+// rows, 32 NT each, whose bank rows stay in registers, and the rows pass by, up to 256 of them copied to LDS as codes before the
+// first product.  A workgroup then writes 512 / NB columns of 32 rows at about the same time, which fills whole lines also where out's rows
+// begin in the middle of one, and waits for no store.  Where the bank has fewer columns, 8 / wc waves share them and take the row tiles in
+// turn.
+constexpr int Q8_PR = 256;  // rows per workgroup, at most
+template <class TT, int NB, bool TAIL>
+__global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int tiles, int cuts, int wc, int rt, typename TT::T *__restrict__ out) {
+  constexpr int NT = 2 / NB;
+  constexpr int RB = Q8_BLOCK * NB;
+  typedef Q8Bank<NB, TAIL, sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR, 1, 1> Rows;
+  __shared__ __align__(16) Rows L;
+  __shared__ __align__(16) uint8_t turn[8][4096];
+  // the column cuts of the same rows follow each other on one XCD (workgroup b runs on XCD b % 8): they share the lines between them
+  const unsigned n = (unsigned)tiles * (unsigned)cuts, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (id >= n) return;
+  Q8Seg S;
+  if (!q8_find<8>(A, id / cuts, 32 * rt, S)) return;
+  const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cols = min(S.n1 - S.n0, A.n_cols), n0 = ((int)(id % cuts) * wc + w % wc) * 32 * NT, m1 = min(S.r1, S.r0 + 32 * rt);
+  if ((int)(id % cuts) * wc * 32 * NT >= cols) return;
+  uint32_t e[Rows::NE];
+  L.copy(0, A.a + (size_t)S.r0 * A.K, A.ae + (size_t)S.r0 * NB, A.K, m1 - S.r0, 0, 32 * rt, tid, e);
+  // The wave's 32 NT bank rows, 8 KB, read in order of addresses and turned in LDS by halves: lanes i < 16 have their rows in the first
+  // (read by rows, a load instruction would touch 32 lines for 32 bytes of each).
+  u4va g[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int r = (64 * j + lane) / (8 * NB), q = (64 * j + lane) % (8 * NB);
+    const size_t row = (size_t)S.n0 + min(n0 + r, cols - 1);
+    g[j] = !TAIL || 16 * q < A.K ? *(const u4va *)(A.b + row * A.K + 16 * q) : u4va{0, 0, 0, 0};
+  }
+  uint32_t ey[NT][NB];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) ey[t][b] = A.be[((size_t)S.n0 + min(n0 + NT * i + t, cols - 1)) * NB + b];
+  Q8Raw raw[NT][NB];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = (64 * j + lane) / (8 * NB), q = (64 * j + lane) % (8 * NB);
+      *(u4va *)&turn[w][r * RB + 16 * (q ^ (r / NT & 7))] = g[4 * half + j];
+    }
+    q8_wave_sync();
+    if ((i >> 4) == half) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) raw[t][b].v[u] = *(const u4va *)&turn[w][(NT * (i & 15) + t) * RB + 16 * ((8 * b + 2 * u + h) ^ (i & 7))];
+    }
+    q8_wave_sync();
+  }
+  Q8Frag y[NT][NB];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) y[t][b] = q8_frag(raw[t][b], q8_scale(ey[t][b]));
+  L.put_scale(0, tid, e);
   q8_wait_copies();
   __syncthreads();
-  for (int c = first; c < chunks; ++c) {
-    if (c + 1 < chunks) e = L.copy(bank, bank_e, A.K, cols, c + 1, tid);
-    const int left = min(cols - c * Q8_SR, Q8_SR);
-    for (int n = 0; n < left; n += 32) {
-      Q8Frag y[NB];
-      L.get(c, n, i, h, A.K, y);
+  if (n0 >= cols) return;
+  for (int m = 32 * (w / wc); S.r0 + m < m1; m += 32 * (8 / wc)) {
+    f16v acc[NT];
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        if (m0 + 32 * t >= S.r1) break;
-        f16v acc = q8_zero();
+    for (int t = 0; t < NT; ++t) acc[t] = q8_zero();
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc = q8_mfma(x[t][b], y[b], acc);
-        q8_store<TT>(out, A.n_cols, m0 + 32 * t, S.r1, c * Q8_SR + n, cols, i, h, acc);
-      }
+    for (int b = 0; b < NB; ++b) {
+      const Q8Frag x = L.get(0, m, b, i, h, A.K);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = q8_mfma(x, y[t][b], acc[t]);
     }
-    if (c + 1 < chunks) L.put_scale(c + 1, tid, e);
-    q8_wait_copies();
-    __syncthreads();
+    q8_store_group<TT, NT>(out, A.n_cols, S.r0 + m, m1, n0, cols, i, h, acc);
   }
 }
 
@@ -533,9 +610,10 @@ __device__ __forceinline__ float q8_max(float best, const f16v &acc) {
 template <int NB, int T>
 __global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Args A, float *__restrict__ out) {
   constexpr int K = Q8_BLOCK * NB;
-  __shared__ __align__(16) Q8Bank<NB, false> L;
+  typedef Q8Bank<NB, false, 128, 2, 1> Bank;  // a chunk of 128 rows is copied while the one before is multiplied: one barrier a chunk
+  __shared__ __align__(16) Bank L;
   Q8Seg S;
-  if (!q8_find<256 * T, 8>(A, blockIdx.x, S)) return;
+  if (!q8_find<8>(A, blockIdx.x, 256 * T, S)) return;
   const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = tid >> 6;
   const int rows = S.n1 - S.n0, m0 = S.r0 + 32 * T * w;
   const uint8_t *bank = A.b + (size_t)S.n0 * K, *bank_e = A.be + (size_t)S.n0 * NB;
@@ -543,7 +621,8 @@ __global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Ar
 #pragma unroll
   for (int t = 0; t < T; ++t) best[t] = -INFINITY;
   if (rows > 0) {
-    uint32_t e = L.copy(bank, bank_e, K, rows, 0, tid);
+    uint32_t e[Bank::NE];
+    L.copy(0, bank, bank_e, K, rows, 0, 128, tid, e);
     Q8Frag x[T][NB];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
@@ -554,14 +633,15 @@ __global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Ar
     L.put_scale(0, tid, e);
     q8_wait_copies();
     __syncthreads();
-    const int chunks = (rows + Q8_SR - 1) / Q8_SR;
+    const int chunks = (rows + 127) / 128;
     for (int c = 0; c < chunks; ++c) {
-      if (c + 1 < chunks) e = L.copy(bank, bank_e, K, rows, c + 1, tid);
+      if (c + 1 < chunks) L.copy((c + 1) & 1, bank, bank_e, K, rows, 128 * (c + 1), 128, tid, e);
       if (m0 < S.r1) {
-        const int left = min(rows - c * Q8_SR, Q8_SR);
+        const int left = min(rows - 128 * c, 128);
         for (int n = 0; n < left; n += 32) {
           Q8Frag y[NB];
-          L.get(c, n, i, h, K, y);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) y[b] = L.get(c & 1, n, b, i, h, K);
 #pragma unroll
           for (int t = 0; t < T; ++t) {
             f16v acc = q8_zero();
@@ -571,7 +651,7 @@ __global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Ar
           }
         }
       }
-      if (c + 1 < chunks) L.put_scale(c + 1, tid, e);
+      if (c + 1 < chunks) L.put_scale((c + 1) & 1, tid, e);
       q8_wait_copies();
       __syncthreads();
     }
@@ -589,7 +669,7 @@ __global__ __launch_bounds__(512) void q8_score_few_kernel(Q8Args A, float *__re
   constexpr int RB = Q8_BLOCK * NB;
   __shared__ float top[8][32];
   Q8Seg S;
-  if (!q8_find<32, 8>(A, blockIdx.x, S)) return;
+  if (!q8_find<8>(A, blockIdx.x, 32, S)) return;
   const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, w = threadIdx.x >> 6;
   const int rows = S.n1 - S.n0;
   float best = -INFINITY;

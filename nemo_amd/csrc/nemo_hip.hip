@@ -1276,6 +1276,11 @@ static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, vo
     else if (A.nb == 1) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, true>), grid, wg, 0, st, A, n, c, wc, rt, out);
     else if (A.K == 256) hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, false>), grid, wg, 0, st, A, n, c, wc, rt, out);
     else hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, true>), grid, wg, 0, st, A, n, c, wc, rt, out);
+  } else if (A.nb > 2 && (size_t)A.M >= 64 * (size_t)A.n_seg && q8_tiles(A, 128) * chunks >= cus / 4) {
+    // Long rows: tiles of 128 x 128, from as many on as occupy a quarter of the compute units.
+    const size_t n = q8_tiles(A, 128), blocks = (n * chunks + 7) / 8 * 8;
+    if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+    hipLaunchKernelGGL((q8_product_long_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, st, A, (int)n, (int)chunks, out);
   } else {
     const size_t few = q8_tiles(A, 32);
     if (few > Q8_MAX_BLOCKS || chunks > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);

@@ -596,6 +596,86 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
   }
 }
 
+// Long rows (K > 256): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step.  The codes of the next step are read into registers while the
+// current one is multiplied out of LDS, and put into the other of two buffers after it: one barrier a step, two workgroups a compute
+// unit.  A step is 32 matrix instructions a wave (1024 cycles) against 128 widening ones and 16 KB out of LDS.
+// LDS: rows of 8 chunks of 16 bytes, chunk c at place c ^ key, key = row & 7 for a and row / 2 & 7 for b, whose rows are read two by two.
+template <class TT>
+__global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
+  __shared__ __align__(16) uint8_t codes[2][2][128 * Q8_BLOCK];  // [buffer][a, b]
+  __shared__ float scale[2][2][128];
+  // the column tiles of the same rows follow each other on one XCD, whose L2 keeps the rows of a
+  const unsigned n = (unsigned)tiles * (unsigned)cuts, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (id >= n) return;
+  Q8Seg S;
+  if (!q8_find<4>(A, id / cuts, 128, S)) return;
+  const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cols = min(S.n1 - S.n0, A.n_cols), n0 = (int)(id % cuts) * 128, m1 = S.r1;
+  if (n0 >= cols) return;
+  // thread's share of a step: 4 chunks of a and of b, rows tid / 8 + 32 j, chunk tid % 8; and one scale
+  const int q = tid & 7, r0 = tid >> 3;
+  const uint8_t *pa[4], *pb[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    pa[j] = A.a + (size_t)min(S.r0 + r0 + 32 * j, m1 - 1) * A.K + 16 * q;
+    pb[j] = A.b + ((size_t)S.n0 + min(n0 + r0 + 32 * j, cols - 1)) * A.K + 16 * q;
+  }
+  const uint8_t *pe = tid < 128 ? A.ae + (size_t)min(S.r0 + tid, m1 - 1) * A.nb : A.be + ((size_t)S.n0 + min(n0 + tid - 128, cols - 1)) * A.nb;
+  u4va ga[4], gb[4];
+  uint32_t ge;
+  auto fetch = [&](int b) {
+    const bool in = b * Q8_BLOCK + 16 * q < A.K;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ga[j] = in ? *(const u4va *)(pa[j] + b * Q8_BLOCK) : u4va{0, 0, 0, 0};
+      gb[j] = in ? *(const u4va *)(pb[j] + b * Q8_BLOCK) : u4va{0, 0, 0, 0};
+    }
+    ge = pe[b];
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = r0 + 32 * j;
+      *(u4va *)&codes[buf][0][r * Q8_BLOCK + 16 * (q ^ (r & 7))] = ga[j];
+      *(u4va *)&codes[buf][1][r * Q8_BLOCK + 16 * (q ^ (r >> 1 & 7))] = gb[j];
+    }
+    scale[buf][tid >> 7][tid & 127] = q8_scale(ge);
+  };
+  auto get = [&](int buf, int which, int row) {
+    Q8Raw raw;
+    const int key = which ? row >> 1 & 7 : row & 7;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) raw.v[u] = *(const u4va *)&codes[buf][which][row * Q8_BLOCK + 16 * ((2 * u + h) ^ key)];
+    return q8_frag(raw, scale[buf][which][row]);
+  };
+  const int mw = 64 * (w >> 1), nw = 64 * (w & 1);  // the wave's corner of the tile
+  f16v acc[2][2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) acc[s][t] = q8_zero();
+  fetch(0);
+  put(0);
+  __syncthreads();
+  for (int b = 0; b < A.nb; ++b) {
+    const int buf = b & 1;
+    if (b + 1 < A.nb) fetch(b + 1);
+    const Q8Frag x0 = get(buf, 0, mw + i), x1 = get(buf, 0, mw + 32 + i);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Q8Frag y = get(buf, 1, nw + 2 * i + t);
+      acc[0][t] = q8_mfma(x0, y, acc[0][t]);
+      acc[1][t] = q8_mfma(x1, y, acc[1][t]);
+    }
+    if (b + 1 < A.nb) put(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    if (S.r0 + mw + 32 * s < m1 && n0 + nw < cols)
+      q8_store_group<TT, 2>(out, A.n_cols, S.r0 + mw + 32 * s, m1, n0 + nw, cols, i, h, acc[s]);
+}
+
 // ---------------------------------------------------------------- clutter score
 // The largest product of a pixel's row with the rows of its image's bank; NaN where one of them is, -infinity for an empty bank.  The
 // bank is the first operand, so a lane's 16 results are of one pixel and the maximum stays in the lane: 8 three-way

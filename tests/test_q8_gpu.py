@@ -140,7 +140,8 @@ def test_offsets_beyond_32_bits(eng):
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('m,n,k', [(1, 1, 16), (1, 1088, 128), (33, 31, 128), (127, 129, 144), (128, 128, 256), (200, 1, 512), (257, 300, 240),
                                    (1000, 77, 128), (129, 260, 2048), (64, 33, 4112),
-                                   (8000, 1088, 128), (33001, 77, 256), (17000, 261, 64), (9001, 1000, 240)])
+                                   (8000, 1088, 128), (33001, 77, 256), (17000, 261, 64), (9001, 1000, 240),
+                                   (8200, 129, 1024), (1000, 1030, 400), (5000, 257, 272)])
 def test_product(eng, m, n, k, dtype):
     (a, a64), (b, b64) = rows8(m, k, m + k), rows8(n, k, n + k + 1)
     got = eng.q8_product(a, b, dtype=dtype)
@@ -192,6 +193,7 @@ def offsets(sizes):
     ([5000, 300, 20000, 7, 0, 8000], [300, 500, 129, 1000, 3, 1], None, 128),
     ([9000, 8500, 300], [1, 515], [1, 1, 0], 256),
     ([12000, 5000], [130, 700], None, 80),
+    ([3000, 129, 0, 2500], [260, 1, 20, 300], [0, 3, 1, 2], 528),
     ([(i * 37) % 90 for i in range(700)], [(i * 13) % 41 for i in range(700)], None, 128),
 ])
 def test_grouped_product(eng, sizes, banks, bank_of, k, dtype):

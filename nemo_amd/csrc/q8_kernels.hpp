@@ -359,6 +359,21 @@ __device__ __forceinline__ void q8_copy16(const uint8_t *from, uint8_t *lds) {
   __builtin_amdgcn_global_load_lds((const uint32_t GAS *)(uintptr_t)from, (__attribute__((address_space(3))) uint32_t *)lds, 16, 0, 0);
 }
 __device__ __forceinline__ void q8_wait_copies() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+// Where chunk q (16 bytes) of a row lies in LDS: lines of 256 bytes hold two rows of 128 or one of 256, piece x of line l at place
+// x ^ (l & 15).  The 16 lanes that are served together read the same chunk of 16 rows, one after another or two apart, and meet 16 different
+// places in the 64 banks either way.
+template <int NB>
+__device__ __forceinline__ int q8_place(int row, int q) {
+  const int l = NB == 1 ? row >> 1 : row, x = NB == 1 ? (row & 1) * 8 + q : q;
+  return l * 256 + 16 * (x ^ (l & 15));
+}
+// and the row and chunk that lie at 16-byte place p
+template <int NB>
+__device__ __forceinline__ void q8_at(int p, int &row, int &q) {
+  const int l = p >> 4, x = (p & 15) ^ (l & 15);
+  row = NB == 1 ? 2 * l + (x >> 3) : l;
+  q = NB == 1 ? x & 7 : x;
+}
 // What the wave's lanes wrote to LDS before, its lanes read after.
 __device__ __forceinline__ void q8_wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -444,9 +459,8 @@ __global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, typename 
 }
 
 // The bank's way to LDS, for the kernels that keep their rows of a in registers (8 waves, K <= 128 NB): SR rows at a time as codes, copied
-// by the memory unit.  A row is 8 NB chunks of 16 bytes, chunk c at place c ^ (row / NT & 7): the copy fills places in order of
-// lanes, and the 8 rows (NT apart) that a read of one chunk touches lie in different banks of the LDS.
-template <int NB, bool TAIL, int SR, int BUFS, int NT>  // TAIL: K is less than 128 NB; NT: rows that a lane reads side by side
+// by the memory unit, which fills places (q8_place) in order of lanes.
+template <int NB, bool TAIL, int SR, int BUFS>  // TAIL: K is less than 128 NB
 struct Q8Bank {
   static constexpr int RB = Q8_BLOCK * NB;                  // bytes of a row in LDS
   static constexpr int PER = SR * RB / (512 * 16);          // 16-byte copies per thread and buffer
@@ -460,7 +474,8 @@ struct Q8Bank {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if (8192 * j >= room * RB) break;
-      const int place = (8 * j + w) * 64 + lane, r = place / (8 * NB), q = (place % (8 * NB)) ^ (r / NT & 7);
+      int r, q;
+      q8_at<NB>((8 * j + w) * 64 + lane, r, q);
       const int row = min(first + r, rows - 1);             // rows past the end repeat the last one
       q8_copy16(bank + (TAIL ? (size_t)row * K + min(16 * q, K - 16) : (size_t)row * RB + 16 * q), &codes[buf][(8 * j + w) * 1024]);
     }
@@ -475,16 +490,16 @@ struct Q8Bank {
     for (int j = 0; j < NE; ++j)
       if (tid + 512 * j < SR * NB) scale[buf][tid + 512 * j] = q8_scale(e[j]);
   }
-  // rows n + NT i, i = 0 .. 31, of a buffer
+  // rows n + i, i = 0 .. 31, of a buffer
   __device__ __forceinline__ Q8Frag get(int buf, int n, int b, int i, int h, int K) const {
     Q8Raw raw;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int q = 8 * b + 2 * u + h;
-      raw.v[u] = *(const u4va *)&codes[buf][(n + NT * i) * RB + 16 * (q ^ (i & 7))];
+      raw.v[u] = *(const u4va *)&codes[buf][q8_place<NB>(n + i, q)];
       if (TAIL && 16 * q >= K) raw.v[u] = u4va{0, 0, 0, 0};
     }
-    return q8_frag(raw, scale[buf][(n + NT * i) * NB + b]);
+    return q8_frag(raw, scale[buf][(n + i) * NB + b]);
   }
 };
 
@@ -526,8 +541,7 @@ constexpr int Q8_PR = 256;  // rows per workgroup, at most
 template <class TT, int NB, bool TAIL>
 __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int tiles, int cuts, int wc, int rt, typename TT::T *__restrict__ out) {
   constexpr int NT = 2 / NB;
-  constexpr int RB = Q8_BLOCK * NB;
-  typedef Q8Bank<NB, TAIL, sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR, 1, 1> Rows;
+  typedef Q8Bank<NB, TAIL, sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR, 1> Rows;
   __shared__ __align__(16) Rows L;
   __shared__ __align__(16) uint8_t turn[8][4096];
   // the column cuts of the same rows follow each other on one XCD (workgroup b runs on XCD b % 8): they share the lines between them
@@ -560,7 +574,7 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = (64 * j + lane) / (8 * NB), q = (64 * j + lane) % (8 * NB);
-      *(u4va *)&turn[w][r * RB + 16 * (q ^ (r / NT & 7))] = g[4 * half + j];
+      *(u4va *)&turn[w][q8_place<NB>(r, q)] = g[4 * half + j];
     }
     q8_wave_sync();
     if ((i >> 4) == half) {
@@ -569,7 +583,7 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) raw[t][b].v[u] = *(const u4va *)&turn[w][(NT * (i & 15) + t) * RB + 16 * ((8 * b + 2 * u + h) ^ (i & 7))];
+          for (int u = 0; u < 4; ++u) raw[t][b].v[u] = *(const u4va *)&turn[w][q8_place<NB>(NT * (i & 15) + t, 8 * b + 2 * u + h)];
     }
     q8_wave_sync();
   }
@@ -596,14 +610,14 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
   }
 }
 
-// Long rows (K > 256): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step.  The codes of the next step are read into registers while the
-// current one is multiplied out of LDS, and put into the other of two buffers after it: one barrier a step, two workgroups a compute
-// unit.  A step is 32 matrix instructions a wave (1024 cycles) against 128 widening ones and 16 KB out of LDS.
-// LDS: rows of 8 chunks of 16 bytes, chunk c at place c ^ key, key = row & 7 for a and row / 2 & 7 for b, whose rows are read two by two.
+// Long rows (K > 256): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS.  There is
+// one buffer: the three workgroups of a compute unit fill each other's waits, which measured better than two buffers and two workgroups
+// (more rows of a on their way at a time).  A step is 32 matrix instructions a wave (1024 cycles) against 128 widening ones and 16 KB out
+// of LDS; the block is multiplied in halves to keep the registers for three.
 template <class TT>
-__global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
-  __shared__ __align__(16) uint8_t codes[2][2][128 * Q8_BLOCK];  // [buffer][a, b]
-  __shared__ float scale[2][2][128];
+__global__ __launch_bounds__(256, 3) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
+  __shared__ __align__(16) uint8_t codes[2][128 * Q8_BLOCK];  // a, b
+  __shared__ float scale[2][128];
   // the column tiles of the same rows follow each other on one XCD, whose L2 keeps the rows of a
   const unsigned n = (unsigned)tiles * (unsigned)cuts, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= n) return;
@@ -612,63 +626,55 @@ __global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int t
   const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cols = min(S.n1 - S.n0, A.n_cols), n0 = (int)(id % cuts) * 128, m1 = S.r1;
   if (n0 >= cols) return;
-  // thread's share of a step: 4 chunks of a and of b, rows tid / 8 + 32 j, chunk tid % 8; and one scale
-  const int q = tid & 7, r0 = tid >> 3;
-  const uint8_t *pa[4], *pb[4];
+  const uint8_t *pa[4], *pb[4];  // the thread's 16-byte pieces of a step, 32 rows apart
+  int r0, q;
+  q8_at<1>(tid, r0, q);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    pa[j] = A.a + (size_t)min(S.r0 + r0 + 32 * j, m1 - 1) * A.K + 16 * q;
-    pb[j] = A.b + ((size_t)S.n0 + min(n0 + r0 + 32 * j, cols - 1)) * A.K + 16 * q;
+    pa[j] = A.a + (size_t)min(S.r0 + r0 + 32 * j, m1 - 1) * A.K;
+    pb[j] = A.b + ((size_t)S.n0 + min(n0 + r0 + 32 * j, cols - 1)) * A.K;
   }
   const uint8_t *pe = tid < 128 ? A.ae + (size_t)min(S.r0 + tid, m1 - 1) * A.nb : A.be + ((size_t)S.n0 + min(n0 + tid - 128, cols - 1)) * A.nb;
-  u4va ga[4], gb[4];
-  uint32_t ge;
-  auto fetch = [&](int b) {
-    const bool in = b * Q8_BLOCK + 16 * q < A.K;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      ga[j] = in ? *(const u4va *)(pa[j] + b * Q8_BLOCK) : u4va{0, 0, 0, 0};
-      gb[j] = in ? *(const u4va *)(pb[j] + b * Q8_BLOCK) : u4va{0, 0, 0, 0};
-    }
-    ge = pe[b];
-  };
-  auto put = [&](int buf) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + 32 * j;
-      *(u4va *)&codes[buf][0][r * Q8_BLOCK + 16 * (q ^ (r & 7))] = ga[j];
-      *(u4va *)&codes[buf][1][r * Q8_BLOCK + 16 * (q ^ (r >> 1 & 7))] = gb[j];
-    }
-    scale[buf][tid >> 7][tid & 127] = q8_scale(ge);
-  };
-  auto get = [&](int buf, int which, int row) {
-    Q8Raw raw;
-    const int key = which ? row >> 1 & 7 : row & 7;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) raw.v[u] = *(const u4va *)&codes[buf][which][row * Q8_BLOCK + 16 * ((2 * u + h) ^ key)];
-    return q8_frag(raw, scale[buf][which][row]);
-  };
   const int mw = 64 * (w >> 1), nw = 64 * (w & 1);  // the wave's corner of the tile
   f16v acc[2][2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int t = 0; t < 2; ++t) acc[s][t] = q8_zero();
-  fetch(0);
-  put(0);
-  __syncthreads();
   for (int b = 0; b < A.nb; ++b) {
-    const int buf = b & 1;
-    if (b + 1 < A.nb) fetch(b + 1);
-    const Q8Frag x0 = get(buf, 0, mw + i), x1 = get(buf, 0, mw + 32 + i);
+    const int k = min(b * Q8_BLOCK + 16 * q, A.K - 16);  // past the end of a row: its last piece, taken for zeros below
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Q8Frag y = get(buf, 1, nw + 2 * i + t);
-      acc[0][t] = q8_mfma(x0, y, acc[0][t]);
-      acc[1][t] = q8_mfma(x1, y, acc[1][t]);
+    for (int j = 0; j < 4; ++j) {
+      q8_copy16(pa[j] + k, &codes[0][4096 * j + 1024 * w]);
+      q8_copy16(pb[j] + k, &codes[1][4096 * j + 1024 * w]);
     }
-    if (b + 1 < A.nb) put(buf ^ 1);
+    scale[tid >> 7][tid & 127] = q8_scale(pe[b]);
+    q8_wait_copies();
     __syncthreads();
+    const int left = A.K - b * Q8_BLOCK;
+    const float s0 = scale[0][mw + i], s1 = scale[0][mw + 32 + i], t0 = scale[1][nw + 2 * i], t1 = scale[1][nw + 2 * i + 1];
+    auto get = [&](int which, int row, int u, float s, bf8v (&v)[2]) {
+      u4va x = *(const u4va *)&codes[which][q8_place<1>(row, 2 * u + h)];
+      if (left < Q8_BLOCK && 16 * (2 * u + h) >= left) x = u4va{0, 0, 0, 0};
+      v[0] = q8_numbers(x[0], x[1], s);
+      v[1] = q8_numbers(x[2], x[3], s);
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      bf8v x0[2], x1[2], y0[2], y1[2];
+      get(0, mw + i, u, s0, x0);
+      get(1, nw + 2 * i, u, t0, y0);
+      get(0, mw + 32 + i, u, s1, x1);
+      get(1, nw + 2 * i + 1, u, t1, y1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0[e], y0[e], acc[0][0], 0, 0, 0);
+        acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1[e], y0[e], acc[1][0], 0, 0, 0);
+        acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0[e], y1[e], acc[0][1], 0, 0, 0);
+        acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1[e], y1[e], acc[1][1], 0, 0, 0);
+      }
+    }
+    __syncthreads();  // nobody reads the buffer any more
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s)
@@ -690,7 +696,7 @@ __device__ __forceinline__ float q8_max(float best, const f16v &acc) {
 template <int NB, int T>
 __global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Args A, float *__restrict__ out) {
   constexpr int K = Q8_BLOCK * NB;
-  typedef Q8Bank<NB, false, 128, 2, 1> Bank;  // a chunk of 128 rows is copied while the one before is multiplied: one barrier a chunk
+  typedef Q8Bank<NB, false, 128, 2> Bank;  // a chunk of 128 rows is copied while the one before is multiplied: one barrier a chunk
   __shared__ __align__(16) Bank L;
   Q8Seg S;
   if (!q8_find<8>(A, blockIdx.x, 256 * T, S)) return;

@@ -53,6 +53,7 @@ class PoseEngine:
             raise _lib.NemoHipError('PoseEngine needs a GPU device; there is no CPU fallback')
         if self.device.index is None:  # 'cuda' -> the current device, so that tensors on cuda:k compare equal
             self.device = torch.device('cuda', torch.cuda.current_device())
+        self._gpu = self.device.index
         torch.cuda.set_device(self.device)
         # index tensors (img_idx / mesh_idx / grid_idx) are range-checked only on request: the check reads
         # them back, i.e. synchronises
@@ -87,6 +88,10 @@ class PoseEngine:
     # ------------------------------------------------------------------ setup
     def _stream(self):
         return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _raw_stream(self):
+        """The current stream of this device as a number."""
+        return torch.cuda.current_stream(self._gpu).cuda_stream
 
     def register_mesh(self, verts, faces, bank) -> int:
         """verts: PRE-PROCESSED [V,3] f32 (x,z,-y); faces [F,3] int; bank [V,D] f32."""
@@ -248,150 +253,166 @@ class PoseEngine:
         return feat, clu
 
     # ------------------------------------------------------------------ rows held in 8 bits (q8.py has the format)
-    _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    # A pass over one image takes the GPU 3 us: the checks below ask each tensor for no more than they need, and addresses go to
+    # the library as plain numbers.
+    def _ready(self, t, dtype, name):
+        """t's address, once t is a contiguous tensor of `dtype` on this device."""
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != self._gpu or not t.is_contiguous():
+            if t is None:
+                raise TypeError(f'{name}: expected a torch tensor')
+            _chk(t, dtype, name, self.device)
+        return t.data_ptr()
 
-    def _q8(self, pair, name, width=None):
-        """(codes, scale) of rows held in 8 bits, on this device, of the shapes that belong together."""
-        codes = _chk(pair[0], torch.float8_e4m3fn, name + ' codes', self.device)
-        scale = _chk(pair[1], torch.float8_e8m0fnu, name + ' scale', self.device)
-        if codes is None or scale is None:
+    def _q8(self, pair, name):
+        """(codes, scale) of rows held in 8 bits -> the codes' shape and both addresses."""
+        if not isinstance(pair, (tuple, list)) or len(pair) != 2:
             raise TypeError(f'{name}: expected (codes, scale)')
-        if codes.dim() < 2 or scale.shape != codes.shape[:-1] + (q8.n_blocks(codes.shape[-1]),):
-            raise ValueError(f'{name}: codes {tuple(codes.shape)} and scale {tuple(scale.shape)} do not belong together')
-        if width is not None and codes.shape[-1] != width:
-            raise ValueError(f'{name}: expected rows of {width} channels, got {codes.shape[-1]}')
-        return codes, scale
+        codes, scale = pair
+        at = self._ready(codes, torch.float8_e4m3fn, name + ' codes'), self._ready(scale, torch.float8_e8m0fnu, name + ' scale')
+        shape = codes.shape
+        if len(shape) < 2 or scale.shape != shape[:-1] + (-(-shape[-1] // q8.BLOCK),):
+            raise ValueError(f'{name}: codes {tuple(shape)} and scale {tuple(scale.shape)} do not belong together')
+        return (shape,) + at
+
+    def _index(self, t, name, n, hi):
+        """Address of an optional int32 [n]; its values are looked at on request only."""
+        if t is None:
+            return None
+        at = self._ready(t, torch.int32, name)
+        if t.shape != (n,):
+            raise ValueError(f'{name}: expected int32 [{n}], got {tuple(t.shape)}')
+        if self.validate_indices and n and (int(t.min()) < 0 or int(t.max()) >= hi):
+            raise ValueError(f'{name}: values in [{int(t.min())}, {int(t.max())}] outside [0, {hi})')
+        return at
 
     def _offsets(self, t, name, end):
-        t = self._i32(t, name)
-        if t is None or t.dim() != 1 or t.shape[0] < 1:
+        """Address and number of pieces of the int32 [n + 1] that cuts `end` rows into n."""
+        if t is None:
             raise ValueError(f'{name}: expected int32 [n + 1]')
+        at = self._ready(t, torch.int32, name)
+        if t.dim() != 1 or t.shape[0] < 1:
+            raise ValueError(f'{name}: expected int32 [n + 1], got {tuple(t.shape)}')
         if self.validate_indices:
             v = t.cpu().numpy()
             if v[0] < 0 or v[-1] > end or (np.diff(v) < 0).any():
                 raise ValueError(f'{name}: must rise from 0 or more to at most {end}')
-        return t
+        return at, t.shape[0] - 1
 
-    def _index(self, t, name, n, hi):
-        t = self._i32(t, name)
-        if t is not None:
-            if tuple(t.shape) != (n,):
-                raise ValueError(f'{name}: expected int32 [{n}], got {tuple(t.shape)}')
-            if self.validate_indices and n and (int(t.min()) < 0 or int(t.max()) >= hi):
-                raise ValueError(f'{name}: values in [{int(t.min())}, {int(t.max())}] outside [0, {hi})')
-        return t
+    def _done(self, rc, what):
+        if rc < 0:
+            _lib.check(self.ctx, rc, what)
+
+    _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
     def quantize(self, x, channel_major=False, slots=None, out=None):
         """nemo_quantize: rows of f32, bf16 or f16 numbers to q8.Q8(codes, scale), channels last.  x is [..., C], or [n, C, ...]
         with channel_major (a backbone's maps).  slots (int32 [n], n = x.shape[0]): image i is written to out[slots[i]], the rest
         of `out` = (codes, scale), a cache of maps, stays as it was; of equal slots the last image stays."""
-        if not isinstance(x, torch.Tensor) or x.dtype not in self._DTYPES:
+        dtype = self._DTYPES.get(getattr(x, 'dtype', None))
+        if dtype is None:
             raise TypeError('x: expected a float32, bfloat16 or float16 tensor')
-        x = _chk(x, x.dtype, 'x', self.device)
-        if x.dim() < (3 if channel_major else 2):
-            raise ValueError(f'x: expected {"[n, C, ...]" if channel_major else "[..., C]"}, got {tuple(x.shape)}')
-        c = x.shape[1] if channel_major else x.shape[-1]
-        image = tuple(x.shape[2:]) if channel_major else tuple(x.shape[1:-1])
-        n = x.shape[0]
-        slots = self._index(slots, 'slots', n, out[0].shape[0] if out is not None else n)
-        if slots is not None and out is None:
-            raise ValueError('slots: pass the cache they index as out')
+        at, shape = self._ready(x, x.dtype, 'x'), x.shape
+        if len(shape) < (3 if channel_major else 2):
+            raise ValueError(f'x: expected {"[n, C, ...]" if channel_major else "[..., C]"}, got {tuple(shape)}')
+        n, c, image = (shape[0], shape[1], shape[2:]) if channel_major else (shape[0], shape[-1], shape[1:-1])
         if out is None:
+            if slots is not None:
+                raise ValueError('slots: pass the cache they index as out')
             out = q8.empty((n,) + image + (c,), self.device)
-        codes, scale = self._q8(out, 'out', c)
-        if codes.shape[1:-1] != image or (slots is None and codes.shape[0] != n):
-            raise ValueError(f'out: codes {tuple(codes.shape)} do not hold {n} images of {image + (c,)}')
-        rows, room = math.prod(image), codes.shape[0]
+        room, codes, scale = self._q8(out, 'out')
+        if room[1:] != image + (c,) or (slots is None and room[0] != n):
+            raise ValueError(f'out: codes {tuple(room)} do not hold {n} images of {tuple(image + (c,))}')
+        rows, n_slots = math.prod(image), room[0]
+        slot_at = self._index(slots, 'slots', n, n_slots)
         if slots is None and not channel_major:   # one run of rows
-            n, rows, room = 1, n * rows, 1
-        _lib.check(self.ctx, self.lib.nemo_quantize(self.ctx, _ptr(x), self._DTYPES[x.dtype], int(channel_major), n, rows, c, _ptr(slots), room,
-                                                    _ptr(codes), _ptr(scale), self._stream()), 'nemo_quantize')
-        return q8.Q8(codes, scale)
+            n, rows, n_slots = 1, n * rows, 1
+        self._done(self.lib.nemo_quantize(self.ctx, at, dtype, channel_major, n, rows, c, slot_at, n_slots, codes, scale, self._raw_stream()),
+                   'nemo_quantize')
+        return q8.Q8(*out)
 
     def dequantize(self, codes, scale, slots=None, channel_major=False, dtype=torch.float32, out=None):
         """nemo_dequantize: rows held in 8 bits back to numbers of `dtype` (of `out`, where that is given): all of them, or the images slots[i]
         (int32) of a cache.  channel_major: images come back as [n, C, ...]."""
-        codes, scale = self._q8((codes, scale), 'x')
+        room, codes_at, scale_at = self._q8((codes, scale), 'x')
+        if channel_major and len(room) < 3:
+            raise ValueError(f'codes: expected [n, ..., C], got {tuple(room)}')
+        n, image, c = room[0], room[1:-1], room[-1]
+        slot_at = None
         if slots is not None:
-            slots = self._index(slots, 'slots', slots.shape[0] if slots.dim() == 1 else -1, codes.shape[0])
-        if channel_major and codes.dim() < 3:
-            raise ValueError(f'codes: expected [n, ..., C], got {tuple(codes.shape)}')
-        n, image, c = codes.shape[0] if slots is None else slots.shape[0], tuple(codes.shape[1:-1]), codes.shape[-1]
+            n = slots.shape[0] if slots.dim() else 0
+            slot_at = self._index(slots, 'slots', n, room[0])
         shape = (n, c) + image if channel_major else (n,) + image + (c,)
-        dtype = out.dtype if out is not None else dtype
-        if dtype not in self._DTYPES:
-            raise TypeError(f'dtype: float32, bfloat16 or float16, got {dtype}')
-        x = self._empty(shape, dtype) if out is None else _chk(out, dtype, 'out', self.device)
-        if tuple(x.shape) != shape:
-            raise ValueError(f'out: expected {shape}, got {tuple(x.shape)}')
-        rows, room = math.prod(image), codes.shape[0]
+        if out is None:
+            out = self._empty(shape, dtype)
+        kind = self._DTYPES.get(out.dtype)
+        if kind is None:
+            raise TypeError(f'dtype: float32, bfloat16 or float16, got {out.dtype}')
+        at = self._ready(out, out.dtype, 'out')
+        if out.shape != shape:
+            raise ValueError(f'out: expected {tuple(shape)}, got {tuple(out.shape)}')
+        rows, n_slots = math.prod(image), room[0]
         if slots is None and not channel_major:
-            n, rows, room = 1, n * rows, 1
-        _lib.check(self.ctx, self.lib.nemo_dequantize(self.ctx, _ptr(codes), _ptr(scale), _ptr(slots), room, n, rows, c, self._DTYPES[dtype],
-                                                      int(channel_major), _ptr(x), self._stream()), 'nemo_dequantize')
-        return x
+            n, rows, n_slots = 1, n * rows, 1
+        self._done(self.lib.nemo_dequantize(self.ctx, codes_at, scale_at, slot_at, n_slots, n, rows, c, kind, channel_major, at,
+                                            self._raw_stream()), 'nemo_dequantize')
+        return out
 
     def _product_out(self, out, shape, dtype, fill):
+        """The result's tensor, address and type; a fresh one is zero where `fill` says that not all of it is written."""
         if out is None:
-            make = torch.zeros if fill else torch.empty
-            out = make(shape, dtype=dtype, device=self.device)
-        elif tuple(out.shape) != shape:
-            raise ValueError(f'out: expected {shape}, got {tuple(out.shape)}')
-        if out.dtype not in (torch.float32, torch.bfloat16):
+            out = (torch.zeros if fill else torch.empty)(shape, dtype=dtype, device=self.device)
+        elif out.shape != shape:
+            raise ValueError(f'out: expected {tuple(shape)}, got {tuple(out.shape)}')
+        if out.dtype is not torch.float32 and out.dtype is not torch.bfloat16:
             raise TypeError(f'out: float32 or bfloat16, got {out.dtype}')
-        return _chk(out, out.dtype, 'out', self.device)
+        return out, self._ready(out, out.dtype, 'out'), self._DTYPES[out.dtype]
 
     def q8_product(self, a, b, dtype=torch.float32, out=None):
         """nemo_q8_product: [..., K] times [N, K] -> [..., N], both (codes, scale); f32 or bf16."""
-        ac, as_ = self._q8(a, 'a')
-        bc, bs = self._q8(b, 'b', ac.shape[-1])
-        if bc.dim() != 2:
-            raise ValueError(f'b: expected [N, K], got {tuple(bc.shape)}')
-        N, K = bc.shape
-        out = self._product_out(out, tuple(ac.shape[:-1]) + (N,), dtype, False)
-        _lib.check(self.ctx, self.lib.nemo_q8_product(self.ctx, _ptr(ac), _ptr(as_), math.prod(ac.shape[:-1]), _ptr(bc), _ptr(bs), N, K, self._DTYPES[out.dtype],
-                                                      _ptr(out), self._stream()), 'nemo_q8_product')
+        (*m, k), ac, ae = self._q8(a, 'a')
+        bshape, bc, be = self._q8(b, 'b')
+        if len(bshape) != 2 or bshape[1] != k:
+            raise ValueError(f'b: expected [N, {k}], got {tuple(bshape)}')
+        out, at, kind = self._product_out(out, (*m, bshape[0]), dtype, False)
+        self._done(self.lib.nemo_q8_product(self.ctx, ac, ae, math.prod(m), bc, be, bshape[0], k, kind, at, self._raw_stream()), 'nemo_q8_product')
         return out
 
     def q8_grouped_product(self, a, row_offsets, b, bank_offsets, bank_of=None, n_cols=None, dtype=torch.float32, out=None):
         """nemo_q8_grouped_product: rows row_offsets[s] .. row_offsets[s + 1] of a [M, K] times rows bank_offsets[g] .. bank_offsets[g + 1] of
         b [N, K], g = bank_of[s] (default s) -> [M, n_cols].  What no product reaches (columns behind a shorter bank, rows of no
         segment) stays as it was in `out`, and is zero without one.  n_cols: at least the longest bank (default: out's, or N)."""
-        ac, as_ = self._q8(a, 'a')
-        bc, bs = self._q8(b, 'b', ac.shape[-1])
-        if ac.dim() != 2 or bc.dim() != 2:
-            raise ValueError(f'expected a [M, K] and b [N, K], got {tuple(ac.shape)} and {tuple(bc.shape)}')
-        (M, K), N = ac.shape, bc.shape[0]
-        row_offsets, bank_offsets = self._offsets(row_offsets, 'row_offsets', M), self._offsets(bank_offsets, 'bank_offsets', N)
-        n_seg, n_banks = row_offsets.shape[0] - 1, bank_offsets.shape[0] - 1
-        bank_of = self._index(bank_of, 'bank_of', n_seg, n_banks)
-        if out is not None and out.dim() == 2 and n_cols is None:
-            n_cols = out.shape[1]
-        out = self._product_out(out, (M, N if n_cols is None else int(n_cols)), dtype, True)
-        _lib.check(self.ctx, self.lib.nemo_q8_grouped_product(
-            self.ctx, _ptr(ac), _ptr(as_), M, _ptr(row_offsets), n_seg, _ptr(bc), _ptr(bs), N, _ptr(bank_offsets), n_banks, _ptr(bank_of), K,
-            self._DTYPES[out.dtype], out.shape[1], _ptr(out), self._stream()), 'nemo_q8_grouped_product')
+        ashape, ac, ae = self._q8(a, 'a')
+        bshape, bc, be = self._q8(b, 'b')
+        if len(ashape) != 2 or len(bshape) != 2 or ashape[1] != bshape[1]:
+            raise ValueError(f'expected a [M, K] and b [N, K], got {tuple(ashape)} and {tuple(bshape)}')
+        (M, K), N = ashape, bshape[0]
+        row_at, n_seg = self._offsets(row_offsets, 'row_offsets', M)
+        bank_at, n_banks = self._offsets(bank_offsets, 'bank_offsets', N)
+        of_at = self._index(bank_of, 'bank_of', n_seg, n_banks)
+        if n_cols is None:
+            n_cols = out.shape[1] if out is not None and out.dim() == 2 else N
+        out, at, kind = self._product_out(out, (M, int(n_cols)), dtype, True)
+        self._done(self.lib.nemo_q8_grouped_product(self.ctx, ac, ae, M, row_at, n_seg, bc, be, N, bank_at, n_banks, of_at, K, kind, out.shape[1], at,
+                                                    self._raw_stream()), 'nemo_q8_grouped_product')
         return out
 
     def q8_clutter_score(self, feat, cbank, bank_offsets=None, bank_of=None, out=None):
         """nemo_q8_clutter_score: clutter_score of maps [n, h, w, D] and vectors [K, D] held in 8 bits, with bank bank_of[i] (int32 [n]) for
         image i: rows bank_offsets[g] .. bank_offsets[g + 1] of cbank.  Without offsets all of cbank is one bank.  -inf for an empty bank;
         images whose bank_of is out of range stay as they were in `out` (zero without one)."""
-        fc, fs = self._q8(feat, 'feat', self.D)
-        bc, bs = self._q8(cbank, 'cbank', self.D)
-        if tuple(fc.shape[1:]) != (self.h, self.w, self.D):
-            raise ValueError(f'feat: expected pixel-major [n_img, {self.h}, {self.w}, {self.D}], got {tuple(fc.shape)}')
-        if bc.dim() != 2:
-            raise ValueError(f'cbank: expected [K, {self.D}], got {tuple(bc.shape)}')
-        n, K, n_banks = fc.shape[0], bc.shape[0], 1
-        if bank_offsets is not None:
-            bank_offsets = self._offsets(bank_offsets, 'bank_offsets', K)
-            n_banks = bank_offsets.shape[0] - 1
-        bank_of = self._index(bank_of, 'bank_of', n, n_banks)
-        out = self._product_out(out, (n, self.h, self.w), torch.float32, bank_of is not None)
-        _lib.check(self.ctx, self.lib.nemo_q8_clutter_score(
-            self.ctx, _ptr(fc), _ptr(fs), n, _ptr(bc), _ptr(bs), K, _ptr(bank_offsets), n_banks, _ptr(bank_of), _ptr(self._f32(out, 'out')),
-            self._stream()), 'nemo_q8_clutter_score')
+        fshape, fc, fe = self._q8(feat, 'feat')
+        bshape, bc, be = self._q8(cbank, 'cbank')
+        if len(fshape) != 4 or fshape[1:] != (self.h, self.w, self.D):
+            raise ValueError(f'feat: expected pixel-major [n_img, {self.h}, {self.w}, {self.D}], got {tuple(fshape)}')
+        if len(bshape) != 2 or bshape[1] != self.D:
+            raise ValueError(f'cbank: expected [K, {self.D}], got {tuple(bshape)}')
+        n, (bank_at, n_banks) = fshape[0], (None, 1) if bank_offsets is None else self._offsets(bank_offsets, 'bank_offsets', bshape[0])
+        of_at = self._index(bank_of, 'bank_of', n, n_banks)
+        out, at, kind = self._product_out(out, (n, self.h, self.w), torch.float32, bank_of is not None)
+        if kind:
+            raise TypeError('out: expected torch.float32')
+        self._done(self.lib.nemo_q8_clutter_score(self.ctx, fc, fe, n, bc, be, bshape[0], bank_at, n_banks, of_at, at, self._raw_stream()),
+                   'nemo_q8_clutter_score')
         return out
 
     def score_fwd_bwd(self, feat, clu, C_, theta, img_idx=None, mesh_idx=None, want_grad=True):

@@ -1188,7 +1188,8 @@ int nemo_quantize(nemo_ctx *ctx, const void *d_x, int32_t dtype, int32_t channel
   const int rc = q8_check_rows(ctx, "nemo_quantize", dtype, n, rows, C, n_slots, d_x, d_q, d_e);
   if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
-  const size_t per = channel_major ? ((size_t)rows + 63) / 64 : ((size_t)rows * nb + 16 * Q8_QU - 1) / (16 * Q8_QU);
+  const size_t px = dtype == NEMO_F32 ? 64 : 128;  // pixels per workgroup of the channel-major kernel
+  const size_t per = channel_major ? ((size_t)rows + px - 1) / px : ((size_t)rows * nb + 16 * Q8_QU - 1) / (16 * Q8_QU);
   const size_t blocks = per * (channel_major ? nb : 1) * n;
   if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_quantize: too many rows for one launch");
   DeviceGuard on(ctx->device);
@@ -1212,7 +1213,7 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
   const int rc = q8_check_rows(ctx, "nemo_dequantize", dtype, n, rows, C, n_slots, d_x, d_q, d_e);
   if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
-  const size_t per = channel_major ? ((size_t)rows + 63) / 64 : ((size_t)rows * (C / 4) + 256 * Q8_DU - 1) / (256 * Q8_DU);
+  const size_t per = channel_major ? ((size_t)rows + 63) / 64 : ((size_t)rows * (C / (dtype == NEMO_F32 ? 4 : 8)) + 256 * Q8_DU - 1) / (256 * Q8_DU);
   const size_t blocks = per * (channel_major ? nb : 1) * n;
   if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_dequantize: too many rows for one launch");
   DeviceGuard on(ctx->device);

@@ -45,16 +45,30 @@ __device__ __forceinline__ void q8_unpack(uint32_t codes, float s, float *x) {
 }
 
 // the three types a row is quantised from and read back to
-struct Q8F32 { typedef float T; static __device__ __forceinline__ float get(float x) { return x; } static __device__ __forceinline__ float put(float x) { return x; } };
+// (at: number s of those that a 4-byte word holds; bits: a number as it is in memory; NAN_BITS: makes any infinity a NaN)
+struct Q8F32 {
+  typedef float T;
+  static constexpr uint32_t NAN_BITS = 0x00400000u;
+  static __device__ __forceinline__ float get(float x) { return x; }
+  static __device__ __forceinline__ float put(float x) { return x; }
+  static __device__ __forceinline__ float at(uint32_t w, int) { return __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+};
 struct Q8BF16 {
   typedef __bf16 T;
+  static constexpr uint32_t NAN_BITS = 0x0040u;
   static __device__ __forceinline__ float get(__bf16 x) { return (float)x; }
   static __device__ __forceinline__ __bf16 put(float x) { return (__bf16)x; }
+  static __device__ __forceinline__ float at(uint32_t w, int s) { return __uint_as_float(s ? w & 0xffff0000u : w << 16); }
+  static __device__ __forceinline__ uint32_t bits(__bf16 x) { return __builtin_bit_cast(uint16_t, x); }
 };
 struct Q8F16 {
   typedef _Float16 T;
+  static constexpr uint32_t NAN_BITS = 0x0200u;
   static __device__ __forceinline__ float get(_Float16 x) { return (float)x; }
   static __device__ __forceinline__ _Float16 put(float x) { return (_Float16)x; }
+  static __device__ __forceinline__ float at(uint32_t w, int s) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(s ? w >> 16 : w & 0xffffu)); }
+  static __device__ __forceinline__ uint32_t bits(_Float16 x) { return __builtin_bit_cast(uint16_t, x); }
 };
 
 // Where image i of a call sits in the cache: slots[i], or i.  -1: nowhere (out of range).
@@ -96,10 +110,11 @@ __global__ __launch_bounds__(256) void q8_quantize_kernel(const typename TT::T *
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = c0 + (F32 ? 64 * h + 4 * lane : 8 * lane + 4 * h);
-      const bool in = blk < blocks && c < C;
-      const typename TT::T *p = x + ((size_t)img * rows + (in ? row : 0)) * C + (in ? c : 0);
+      typedef typename TT::T v4 __attribute__((ext_vector_type(4)));
+      v4 p = {};
+      if (blk < blocks && c < C) p = *(const v4 *)(x + ((size_t)img * rows + row) * C + c);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[u][4 * h + k] = in ? TT::get(p[k]) : 0.0f;
+      for (int k = 0; k < 4; ++k) v[u][4 * h + k] = TT::get(p[k]);
     }
   }
 #pragma unroll
@@ -141,86 +156,133 @@ __global__ __launch_bounds__(256) void q8_quantize_kernel(const typename TT::T *
 }
 
 // ---------------------------------------------------------------- quantise, pixels contiguous
-// x [n][C][rows] -> the same q and e (the layout a backbone leaves and a feature record holds).  A workgroup owns 64 pixels and one
-// block of 128 channels, a wave 32 of the channels: a lane's 32 numbers are of one pixel, so the maximum needs one exchange
-// between the waves; the codes go through LDS so that a pixel's 128 bytes leave as one line.
+// x [n][C][rows] -> the same q and e (the layout a backbone leaves and a feature record holds).  A workgroup owns 64 PX pixels and one
+// block of 128 channels, a wave 32 of the channels: a lane's numbers are of PX pixels (one 4-byte load a channel: PX = 1 for fp32, 2 for
+// 16 bits, where loads of 2 bytes reached 2.3 TB/s), so the maximum needs one exchange between the waves; the codes go through LDS so that a
+// pixel's 128 bytes leave as one line.
 template <class TT>
 __global__ __launch_bounds__(256) void q8_quantize_t_kernel(const typename TT::T *__restrict__ x, int n, int rows, int C, int nb, unsigned tiles,
                                                             const int32_t *__restrict__ slots, int n_slots, uint8_t *__restrict__ q,
                                                             uint8_t *__restrict__ e) {
-  __shared__ uint32_t top[4][64];
-  __shared__ __align__(16) uint8_t codes[64][Q8_BLOCK + 16];
+  typedef typename TT::T T;
+  constexpr int PX = 4 / (int)sizeof(T), TP = 64 * PX;
+  struct __attribute__((packed, aligned(sizeof(T)))) Word { uint32_t v; };
+  __shared__ uint32_t top[4][TP];
+  __shared__ __align__(16) uint8_t codes[TP][Q8_BLOCK + 16];
   const unsigned per = tiles * (unsigned)nb;
   const int img = (int)(blockIdx.x / per);
   const unsigned rest = blockIdx.x - (unsigned)img * per;
-  const int b = (int)(rest / tiles), p0 = (int)(rest - (unsigned)b * tiles) * 64;
+  const int b = (int)(rest / tiles), p0 = (int)(rest - (unsigned)b * tiles) * TP;
   const int slot = q8_slot(slots, img, n_slots);
   if (slot < 0 || q8_overwritten(slots, img, n, slot)) return;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c0 = b * Q8_BLOCK + 32 * w, p = min(p0 + lane, rows - 1);
-  const typename TT::T *xp = x + (size_t)img * C * rows + p;
-  float v[32];
-  uint32_t m = 0;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int c0 = b * Q8_BLOCK + 32 * w;
+  const T *xp = x + ((size_t)img * C + c0) * rows;
+  uint32_t raw[32];  // PX numbers of channel c0 + k each, as they are in memory
 #pragma unroll
-  for (int k = 0; k < 32; ++k) v[k] = c0 + k < C ? TT::get(xp[(size_t)(c0 + k) * rows]) : 0.0f;
-#pragma unroll
-  for (int k = 0; k < 32; ++k) m = max(m, q8_abs_bits(v[k]));
-  if (__any(m >= Q8_INF)) {
-    m = 0;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const uint32_t a = q8_abs_bits(v[k]);
-      m = max(m, a < Q8_INF ? a : 0u);
-      v[k] = a < Q8_INF ? v[k] : __uint_as_float(0x7fc00000u);
-    }
-  }
-  top[w][lane] = m;
-  __syncthreads();
-  m = max(max(top[0][lane], top[1][lane]), max(top[2][lane], top[3][lane]));
-  const int ex = q8_exponent(m);
-  const float s = q8_pow2(-ex);
+  for (int k = 0; k < 32; ++k) raw[k] = 0;
 #pragma unroll
   for (int k = 0; k < 32; k += 16) {
-    u4va c;
+    if (c0 + k >= C) break;
+    if (p0 + TP <= rows) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = q8_pack(v[k + 4 * j] * s, v[k + 4 * j + 1] * s, v[k + 4 * j + 2] * s, v[k + 4 * j + 3] * s);
-    *(u4va *)&codes[lane][32 * w + k] = c;
+      for (int j = k; j < k + 16; ++j) raw[j] = ((const Word *)(xp + (size_t)j * rows + (p0 + PX * lane)))->v;
+    } else {
+#pragma unroll
+      for (int j = k; j < k + 16; ++j)
+#pragma unroll
+        for (int s = 0; s < PX; ++s) raw[j] |= TT::bits(xp[(size_t)j * rows + min(p0 + PX * lane + s, rows - 1)]) << (16 * s);
+    }
+  }
+  uint32_t m[PX];
+  bool odd = false;
+#pragma unroll
+  for (int s = 0; s < PX; ++s) {
+    m[s] = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) m[s] = max(m[s], q8_abs_bits(TT::at(raw[k], s)));
+    odd |= m[s] >= Q8_INF;
+  }
+  if (__any(odd)) {  // numbers that are not finite: rare, the maxima are taken again without them
+#pragma unroll
+    for (int s = 0; s < PX; ++s) {
+      m[s] = 0;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const uint32_t a = q8_abs_bits(TT::at(raw[k], s));
+        m[s] = max(m[s], a < Q8_INF ? a : 0u);
+        if (a >= Q8_INF) raw[k] |= TT::NAN_BITS << (16 * s);  // infinity to NaN
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < PX; ++s) top[w][PX * lane + s] = m[s];
+  __syncthreads();
+  int ex[PX];
+#pragma unroll
+  for (int s = 0; s < PX; ++s) {
+    const int p = PX * lane + s;
+    ex[s] = q8_exponent(max(max(top[0][p], top[1][p]), max(top[2][p], top[3][p])));
+    const float f = q8_pow2(-ex[s]);
+#pragma unroll
+    for (int k = 0; k < 32; k += 16) {
+      u4va c;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t *r = raw + k + 4 * j;
+        c[j] = q8_pack(TT::at(r[0], s) * f, TT::at(r[1], s) * f, TT::at(r[2], s) * f, TT::at(r[3], s) * f);
+      }
+      *(u4va *)&codes[p][32 * w + k] = c;
+    }
   }
   __syncthreads();
   const size_t row0 = (size_t)slot * rows + p0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < 2 * PX; ++j) {
     const int i = (int)threadIdx.x + 256 * j, r = i >> 3, c = (i & 7) * 16;
     if (p0 + r < rows && b * Q8_BLOCK + c < C) *(u4va *)(q + (row0 + r) * C + (size_t)b * Q8_BLOCK + c) = *(const u4va *)&codes[r][c];
   }
-  if (w == 0 && p0 + lane < rows) e[(row0 + lane) * nb + b] = (uint8_t)(ex + 127);
+  if (w == 0)
+#pragma unroll
+    for (int s = 0; s < PX; ++s)
+      if (p0 + PX * lane + s < rows) e[(row0 + PX * lane + s) * nb + b] = (uint8_t)(ex[s] + 127);
 }
 
 // ---------------------------------------------------------------- read back, channels contiguous
-// q [slot][rows][C], e -> x [n][rows][C]; a lane reads 4 codes and writes 4 numbers, Q8_DU times.  An image without a slot reads zeros.
+// q [slot][rows][C], e -> x [n][rows][C]; a lane reads as many codes as make 16 bytes of numbers, Q8_DU times.  An image without a slot
+// reads zeros.
 constexpr int Q8_DU = 4;
 template <class TT>
 __global__ __launch_bounds__(256) void q8_dequantize_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ e, int rows, int C, int nb,
                                                             unsigned chunks, const int32_t *__restrict__ slots, int n_slots,
                                                             typename TT::T *__restrict__ x) {
-  typedef typename TT::T v4 __attribute__((ext_vector_type(4)));
+  constexpr int P = 16 / (int)sizeof(typename TT::T);
+  typedef typename TT::T vp __attribute__((ext_vector_type(P)));
+  typedef uint32_t cp __attribute__((ext_vector_type(P / 4)));
   const int img = (int)(blockIdx.x / chunks);
   const unsigned chunk = blockIdx.x - (unsigned)img * chunks;
   const int slot = q8_slot(slots, img, n_slots);
-  const size_t quads = (size_t)rows * (C / 4), base = (size_t)max(slot, 0) * rows;
-  const unsigned qpr = (unsigned)C / 4;  // quads per row
+  const unsigned ppr = (unsigned)C / P;  // pieces per row
+  const size_t pieces = (size_t)rows * ppr, base = (size_t)max(slot, 0) * rows;
 #pragma unroll
   for (int u = 0; u < Q8_DU; ++u) {
     const size_t i = (size_t)chunk * (256 * Q8_DU) + 256 * u + threadIdx.x;
-    if (i >= quads) return;
-    const size_t row = i / qpr;
-    const unsigned c4 = (unsigned)(i - row * qpr);
-    float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (slot >= 0) q8_unpack(*(const uint32_t *)(q + base * C + 4 * i), q8_scale(e[(base + row) * nb + c4 / 32]), f);
-    v4 o;
+    if (i >= pieces) return;
+    const size_t row = i / ppr;
+    const unsigned c = (unsigned)(i - row * ppr);
+    float f[P];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = TT::put(f[k]);
-    *(v4 *)(x + (size_t)img * rows * C + 4 * i) = o;
+    for (int k = 0; k < P; ++k) f[k] = 0.0f;
+    if (slot >= 0) {
+      const cp codes = *(const cp *)(q + base * C + P * i);
+      const float s = q8_scale(e[(base + row) * nb + c / (Q8_BLOCK / P)]);
+#pragma unroll
+      for (int k = 0; k < P / 4; ++k) q8_unpack(codes[k], s, f + 4 * k);
+    }
+    vp o;
+#pragma unroll
+    for (int k = 0; k < P; ++k) o[k] = TT::put(f[k]);
+    *(vp *)(x + (size_t)img * rows * C + P * i) = o;
   }
 }
 

@@ -17,6 +17,10 @@ from . import _lib, q8
 from .synthetic import adam_table, ndc_scale
 
 
+# torch.cuda.current_stream(d).cuda_stream without the Stream object in between (1.1 us of a call)
+_raw_current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else C.c_void_p(t.data_ptr())
 
@@ -91,7 +95,7 @@ class PoseEngine:
 
     def _raw_stream(self):
         """The current stream of this device as a number."""
-        return torch.cuda.current_stream(self._gpu).cuda_stream
+        return _raw_current_stream(self._gpu)
 
     def register_mesh(self, verts, faces, bank) -> int:
         """verts: PRE-PROCESSED [V,3] f32 (x,z,-y); faces [F,3] int; bank [V,D] f32."""

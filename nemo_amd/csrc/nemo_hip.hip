@@ -1213,15 +1213,15 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
   const int rc = q8_check_rows(ctx, "nemo_dequantize", dtype, n, rows, C, n_slots, d_x, d_q, d_e);
   if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
-  const size_t per = channel_major ? ((size_t)rows + 63) / 64 : ((size_t)rows * (C / (dtype == NEMO_F32 ? 4 : 8)) + 256 * Q8_DU - 1) / (256 * Q8_DU);
+  const size_t per = channel_major ? ((size_t)rows + 255) / 256 : ((size_t)rows * (C / (dtype == NEMO_F32 ? 4 : 8)) + 256 * Q8_DU - 1) / (256 * Q8_DU);
   const size_t blocks = per * (channel_major ? nb : 1) * n;
   if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_dequantize: too many rows for one launch");
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
 #define Q8_LAUNCH(TT)                                                                                                             \
   if (channel_major)                                                                                                              \
-    hipLaunchKernelGGL((q8_dequantize_t_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, d_e, rows, C, nb, (unsigned)per, \
-                       d_slots, n_slots, (TT::T *)d_x);                                                                          \
+    hipLaunchKernelGGL((q8_dequantize_t_kernel<TT>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(256), 0, (hipStream_t)stream, d_q, d_e, rows, C, nb, \
+                       (unsigned)per, (unsigned)blocks, d_slots, n_slots, (TT::T *)d_x);                                                                          \
   else                                                                                                                            \
     hipLaunchKernelGGL((q8_dequantize_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, d_q, d_e, rows, C, nb, (unsigned)per, \
                        d_slots, n_slots, (TT::T *)d_x)

@@ -287,38 +287,64 @@ __global__ __launch_bounds__(256) void q8_dequantize_kernel(const uint8_t *__res
 }
 
 // ---------------------------------------------------------------- read back, pixels contiguous
-// q [slot][rows][C], e -> x [n][C][rows]: 64 pixels x 128 channels through LDS.
+// q [slot][rows][C], e -> x [n][C][rows]: 256 pixels x 128 channels through LDS, whose rows of 33 words let the lanes of a wave read one word
+// each of different pixels.  A lane writes PX numbers of a channel, the waves neighbouring pixels: 1 KB (fp32) or 512 bytes of a channel
+// leave at about the same time, and the tiles of a channel follow each other on one XCD (workgroup b runs on XCD b % 8), because lines that
+// are filled in parts cost the memory several times their bytes.
 template <class TT>
 __global__ __launch_bounds__(256) void q8_dequantize_t_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ e, int rows, int C, int nb,
-                                                              unsigned tiles, const int32_t *__restrict__ slots, int n_slots,
+                                                              unsigned tiles, unsigned n_blocks, const int32_t *__restrict__ slots, int n_slots,
                                                               typename TT::T *__restrict__ x) {
-  __shared__ uint32_t codes[64][Q8_BLOCK / 4 + 1];
+  typedef typename TT::T T;
+  constexpr int PX = 4 / (int)sizeof(T), TP = 256, WP = 4 / PX;  // WP waves side by side, PX of them share the channels
+  struct __attribute__((packed, aligned(sizeof(T)))) Word { T v[PX]; };
+  __shared__ uint32_t codes[TP][Q8_BLOCK / 4 + 1];
+  const unsigned share = (n_blocks + 7) / 8, id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+  if (id >= n_blocks) return;
   const unsigned per = tiles * (unsigned)nb;
-  const int img = (int)(blockIdx.x / per);
-  const unsigned rest = blockIdx.x - (unsigned)img * per;
-  const int b = (int)(rest / tiles), p0 = (int)(rest - (unsigned)b * tiles) * 64;
+  const int img = (int)(id / per);
+  const unsigned rest = id - (unsigned)img * per;
+  const int b = (int)(rest / tiles), p0 = (int)(rest - (unsigned)b * tiles) * TP;
   const int slot = q8_slot(slots, img, n_slots);
   const size_t row0 = (size_t)max(slot, 0) * rows + p0;
+  u4va v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int i = (int)threadIdx.x + 256 * j, r = i >> 5, c = i & 31;
-    uint32_t v = 0;
-    if (slot >= 0 && p0 + r < rows && b * Q8_BLOCK + 4 * c < C) v = *(const uint32_t *)(q + (row0 + r) * C + (size_t)b * Q8_BLOCK + 4 * c);
-    codes[r][c] = v;
+    const int i = (int)threadIdx.x + 256 * j, r = i >> 3, c = (i & 7) * 16;
+    v[j] = u4va{0, 0, 0, 0};
+    if (slot >= 0 && p0 + r < rows && b * Q8_BLOCK + c < C) v[j] = *(const u4va *)(q + (row0 + r) * C + (size_t)b * Q8_BLOCK + c);
   }
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const float s = slot >= 0 && p0 + lane < rows ? q8_scale(e[(row0 + lane) * nb + b]) : 0.0f;
-  __syncthreads();
-  if (p0 + lane >= rows) return;
-  typename TT::T *xp = x + ((size_t)img * C + b * Q8_BLOCK) * rows + p0 + lane;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), p = (w % WP) * 64 * PX + PX * lane;
+  float s[PX];
+#pragma unroll
+  for (int k = 0; k < PX; ++k) s[k] = slot >= 0 && p0 + p + k < rows ? q8_scale(e[(row0 + p + k) * nb + b]) : 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int c = 32 * w + 4 * j;
-    if (b * Q8_BLOCK + c >= C) break;
-    float f[4];
-    q8_unpack(codes[lane][c / 4], s, f);
+    const int i = (int)threadIdx.x + 256 * j;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) xp[(size_t)(c + k) * rows] = TT::put(f[k]);
+    for (int k = 0; k < 4; ++k) codes[i >> 3][(i & 7) * 4 + k] = v[j][k];
+  }
+  __syncthreads();
+  if (p0 + p >= rows) return;
+  const bool whole = p0 + p + PX <= rows;
+  T *xp = x + ((size_t)img * C + b * Q8_BLOCK) * rows + p0 + p;
+  constexpr int CH_W = Q8_BLOCK / PX;  // channels of a wave
+#pragma unroll
+  for (int j = 0; j < CH_W; j += 4) {
+    const int c = CH_W * (w / WP) + j;
+    if (b * Q8_BLOCK + c >= C) break;
+    float f[PX][4];
+#pragma unroll
+    for (int k = 0; k < PX; ++k) q8_unpack(codes[p + k][c / 4], s[k], f[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      Word o;
+#pragma unroll
+      for (int m = 0; m < PX; ++m) o.v[m] = TT::put(f[m][k]);
+      T *to = xp + (size_t)(c + k) * rows;
+      if (whole) *(Word *)to = o;
+      else *to = o.v[0];
+    }
   }
 }
 

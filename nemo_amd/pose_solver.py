@@ -11,11 +11,12 @@ Function names follow the reference script where a counterpart exists.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, NamedTuple, Optional, Sequence, Union
 
 import numpy as np
 import torch
 
+from . import q8
 from . import synthetic as syn
 from .camera_params import cal_err, cal_rotation_matrix, pose_error  # noqa: F401  (re-exported)
 from .engine import PoseEngine
@@ -128,6 +129,12 @@ class SolveResult:
                             torch.zeros_like(self.loss)], dim=1).contiguous()
 
 
+class ClutterBanks8(NamedTuple):
+    """Clutter vectors of several groups held in 8 bits, one group behind the other (BatchPoseSolver.clutter_banks8)."""
+    vectors: q8.Q8           # [sum K, D]
+    offsets: torch.Tensor    # int32 [groups + 1]
+
+
 class BatchPoseSolver:
     """Batched MeshPoseSolveAll: one PoseEngine, one mesh + pose grid per
     subtype/category, jobs = (image, mesh)."""
@@ -175,11 +182,29 @@ class BatchPoseSolver:
         """normalize(mean(clutter_bank, 0)) (code/MeshPoseSolveAll.py:207) -> [1, D]."""
         return normalize(torch.mean(clutter_bank, dim=0)).unsqueeze(0).contiguous()
 
-    def clutter_scores_by_group(self, feats: torch.Tensor, group_of_image: Sequence[int],
-                                clutter_of_group: Sequence[torch.Tensor]) -> torch.Tensor:
+    def clutter_banks8(self, clutter_of_group: Sequence[torch.Tensor]) -> ClutterBanks8:
+        """The groups' clutter vectors [K_g, D], packed and quantised once for clutter_scores_by_group on 8-bit maps."""
+        if not len(clutter_of_group) or any(c.dim() != 2 or c.shape[0] < 1 for c in clutter_of_group):
+            raise ValueError('clutter_banks8: every group needs at least one clutter vector [K, D]')
+        offsets = np.cumsum([0] + [c.shape[0] for c in clutter_of_group])
+        return ClutterBanks8(self.engine.quantize(torch.cat([c.to(self.device) for c in clutter_of_group]).contiguous()),
+                             torch.as_tensor(offsets, dtype=torch.int32).to(self.device))
+
+    def clutter_scores_by_group(self, feats: Union[torch.Tensor, q8.Q8], group_of_image: Sequence[int],
+                                clutter_of_group: Union[Sequence[torch.Tensor], ClutterBanks8]) -> torch.Tensor:
         """Clutter score maps [n_img,h,w] when images of different subtypes use different clutter banks
-        (code/MeshPoseSolveAll.py:203-207 reads `clutter_<subtype>` inside the subtype loop): images are
-        scored in runs of equal group, each run against its own [K,D] bank."""
+        (code/MeshPoseSolveAll.py:203-207 reads `clutter_<subtype>` inside the subtype loop).  Maps in f32 are
+        scored in runs of equal group, each run against its own [K,D] bank; maps held in 8 bits in one launch, in
+        whatever order their groups come (nemo_q8_clutter_score; the clutter vectors are held in 8 bits too)."""
+        if isinstance(feats, q8.Q8):
+            banks = clutter_of_group if isinstance(clutter_of_group, ClutterBanks8) else self.clutter_banks8(clutter_of_group)
+            group = np.asarray(group_of_image)
+            if group.shape != (feats.codes.shape[0],) or (len(group) and (group.min() < 0 or group.max() >= banks.offsets.shape[0] - 1)):
+                raise ValueError('group_of_image: expected a group of [0, %d) for each of %d images'
+                                 % (banks.offsets.shape[0] - 1, feats.codes.shape[0]))
+            out = torch.empty((len(group), self.geo.h, self.geo.w), dtype=torch.float32, device=self.device)
+            return self.engine.q8_clutter_score(feats, banks.vectors, banks.offsets,
+                                                torch.as_tensor(group, dtype=torch.int32).to(self.device), out=out)
         g = np.asarray(group_of_image)
         clu = torch.empty((feats.shape[0], self.geo.h, self.geo.w), dtype=torch.float32, device=self.device)
         start = 0
@@ -191,13 +216,19 @@ class BatchPoseSolver:
             start = stop
         return clu
 
-    def solve_all(self, feats: torch.Tensor, clutter: Optional[torch.Tensor], mesh_idx: Optional[torch.Tensor] = None,
+    def solve_all(self, feats: Union[torch.Tensor, q8.Q8], clutter: Optional[torch.Tensor], mesh_idx: Optional[torch.Tensor] = None,
                   img_idx: Optional[torch.Tensor] = None, want_trace=False,
                   clutter_scores: Optional[torch.Tensor] = None) -> SolveResult:
         """feats [n_img,h,w,D] pixel-major f32 on the device; clutter [K,D] (K=1: the reference's
         mean vector; K>1: max over the K vectors, lib/MeshUtils.py:273-275) or, instead, ready-made
-        clutter_scores [n_img,h,w] (clutter_scores_by_group); jobs default to image i with mesh mesh_idx[i]."""
+        clutter_scores [n_img,h,w] (clutter_scores_by_group); jobs default to image i with mesh mesh_idx[i].
+        feats may be held in 8 bits (engine.quantize, FeatureRecord.upload8): the clutter score reads them as they
+        are, the grid search and the solve the numbers they stand for, f32 for the length of this call."""
         eng = self.engine
+        if isinstance(feats, q8.Q8):
+            if not self.cfg.turn_off_clutter and clutter_scores is None:
+                clutter_scores = eng.q8_clutter_score(feats, eng.quantize(clutter.reshape(-1, eng.D).contiguous()))
+            feats = eng.dequantize(*feats)
         if self.cfg.turn_off_clutter:
             clu = None
         elif clutter_scores is not None:

@@ -4,6 +4,9 @@
   code/MeshPoseSolveAll.py:173,199-218): one .npz per category with
   ``memory_<subtype>`` [n_vertices, D], ``clutter_<subtype>`` [n_noise, D],
   ``names_<subtype>`` (image names) and one ``<image name>`` -> [D, h, w] f32 map per image;
+  A record held in 8 bits (quantize_record; no counterpart in the reference) has ``features_8bit`` = (h, w, D) and stores
+  every image as u8 [h w (D + ceil(D / 128))]: the pixel-major codes, then the scale bytes (q8.py) -- a quarter of the
+  bytes to read and copy;
 * annotation (one .npz per image, code/MeshPoseSolveAll.py:256-258,270): theta, elevation,
   azimuth, distance, cad_index;
 * per-category error record (code/MeshPoseSolveAll.py:273-274) and the accuracy table of
@@ -26,6 +29,7 @@ from typing import Dict, Iterable, List, Optional, Sequence
 import numpy as np
 import torch
 
+from . import q8
 from .camera_params import cal_err, cal_rotation_matrix
 
 CATEGORIES = ['aeroplane', 'bicycle', 'boat', 'bottle', 'bus', 'car', 'chair', 'diningtable', 'motorbike', 'sofa',
@@ -42,8 +46,12 @@ class FeatureRecord:
         self._z = np.load(path, allow_pickle=False)
         keys = list(self._z.files)
         self.subtypes = sorted(k[len('memory_'):] for k in keys if k.startswith('memory_'))
-        meta = {p + s for s in self.subtypes for p in ('memory_', 'clutter_', 'names_')}
+        meta = {p + s for s in self.subtypes for p in ('memory_', 'clutter_', 'names_')} | {'features_8bit'}
         self.image_keys = [k for k in keys if k not in meta]
+        # (h, w, D) of the maps of a record held in 8 bits, else None
+        self.shape8 = tuple(int(v) for v in self._z['features_8bit']) if 'features_8bit' in keys else None
+        if self.shape8 is not None and (len(self.shape8) != 3 or min(self.shape8) < 1):
+            raise ValueError('%s: features_8bit is not (h, w, D)' % path)
 
     def memory(self, subtype: str) -> np.ndarray:
         return np.ascontiguousarray(self._z['memory_%s' % subtype], dtype=np.float32)
@@ -55,12 +63,29 @@ class FeatureRecord:
         return [str(n) for n in np.asarray(self._z['names_%s' % subtype]).ravel().tolist()]
 
     def feature(self, name: str) -> np.ndarray:
-        """[D, h, w] f32, the layout ExtractFeatures.py:166-168 stores."""
-        return np.asarray(self._z[name], dtype=np.float32)
+        """[D, h, w] f32, the layout ExtractFeatures.py:166-168 stores (of an 8-bit record: the numbers the codes stand for)."""
+        if self.shape8 is None:
+            return np.asarray(self._z[name], dtype=np.float32)
+        return np.ascontiguousarray(q8.dequantize_host(self.feature8(name)).permute(2, 0, 1).numpy())
+
+    def _size8(self):
+        h, w, D = self.shape8
+        return h * w * D, h * w * q8.n_blocks(D)
+
+    def feature8(self, name: str) -> q8.Q8:
+        """Pixel-major map [h, w, D] held in 8 bits, as an 8-bit record stores it."""
+        if self.shape8 is None:
+            raise ValueError('%s is not held in 8 bits' % self.path)
+        (h, w, D), (nc, ns) = self.shape8, self._size8()
+        v = np.asarray(self._z[name])
+        if v.dtype != np.uint8 or v.shape != (nc + ns,):
+            raise ValueError('feature map %r has shape %s of %s, expected %d bytes' % (name, v.shape, v.dtype, nc + ns))
+        v = torch.from_numpy(np.array(v))
+        return q8.Q8(v[:nc].view(h, w, D).view(torch.float8_e4m3fn), v[nc:].view(h, w, q8.n_blocks(D)).view(torch.float8_e8m0fnu))
 
     # ---- direct reads: np.savez stores members uncompressed, so a map's bytes sit in the file as they are
     def _layout(self, name: str):
-        """(byte offset of the array data in the .npz, shape) of a STORED little-endian f32 C-order member, else None
+        """(byte offset of the array data in the .npz, shape) of a STORED little-endian f32 (8-bit record: u8) C-order member, else None
         (compressed record, other dtype: the caller falls back to the zipfile path)."""
         if not hasattr(self, '_zinfo'):
             with zipfile.ZipFile(self.path) as zf:
@@ -80,7 +105,7 @@ class FeatureRecord:
                 version = np.lib.format.read_magic(fh)
                 shape, fortran, dtype = (np.lib.format.read_array_header_1_0(fh) if version == (1, 0)
                                          else np.lib.format.read_array_header_2_0(fh))
-                if dtype == np.dtype('<f4') and not fortran:
+                if dtype == np.dtype('u1' if self.shape8 is not None else '<f4') and not fortran:
                     lay = (fh.tell(), tuple(shape))
         self._layouts[name] = lay
         return lay
@@ -89,7 +114,7 @@ class FeatureRecord:
         """Fill `dst` ([D, h, w] f32, C-contiguous; e.g. a view of pinned memory) with the map `name`: a straight
         pread of the member's bytes when the record is uncompressed (no intermediate copy, no CRC pass), else
         through the zip reader."""
-        lay = self._layout(name)
+        lay = self._layout(name) if self.shape8 is None else None
         if lay is None:
             f = self.feature(name)
             if f.shape != dst.shape:
@@ -111,18 +136,40 @@ class FeatureRecord:
         if own:
             fd = os.open(self.path, os.O_RDONLY)
         try:
-            view = memoryview(dst).cast('B')
-            done = 0
-            while done < len(view):
-                n = os.preadv(fd, [view[done:]], off + done)
-                if n <= 0:
-                    raise IOError('short read of %r in %s' % (name, self.path))
-                done += n
+            self._pread(fd, name, dst, off)
         finally:
             if own:
                 os.close(fd)
 
+    def _pread(self, fd: int, name: str, dst: np.ndarray, off: int) -> None:
+        view = memoryview(dst).cast('B')
+        done = 0
+        while done < len(view):
+            n = os.preadv(fd, [view[done:]], off + done)
+            if n <= 0:
+                raise IOError('short read of %r in %s' % (name, self.path))
+            done += n
+
+    def read_feature8_into(self, name: str, codes: np.ndarray, scale: np.ndarray, fd: int) -> None:
+        """Fill `codes` (u8, h w D bytes) and `scale` (u8) with the map `name` of an 8-bit record: two preads, or the zip reader
+        where the record is compressed."""
+        lay = self._layout(name)
+        if lay is None:
+            f = self.feature8(name)
+            codes.reshape(-1)[:] = f.codes.view(torch.uint8).numpy().reshape(-1)
+            scale.reshape(-1)[:] = f.scale.view(torch.uint8).numpy().reshape(-1)
+            return
+        off, shape = lay
+        if shape != (codes.size + scale.size,):
+            raise ValueError('feature map %r has shape %s, expected %d bytes' % (name, shape, codes.size + scale.size))
+        self._pread(fd, name, codes, off)
+        self._pread(fd, name, scale, off + codes.size)
+
     def feature_shape(self, name: str):
+        """(D, h, w)"""
+        if self.shape8 is not None:
+            h, w, D = self.shape8
+            return D, h, w
         lay = self._layout(name)
         return lay[1] if lay is not None else tuple(self.feature(name).shape)
 
@@ -145,7 +192,13 @@ class FeatureRecord:
         file) would not start before that solve ends and would hold its pinned buffer until then -- pinned copies are
         not slowed by a running solve (57 GB/s either way), whereas copies from pageable memory, a mapping of the
         file included, drop from 41-48 to 7.6 GB/s under one (tools/from_files_breakdown.py).  The host never holds
-        a transposed copy.  stats (optional dict) receives read / wait times and the byte count."""
+        a transposed copy.  stats (optional dict) receives read / wait times and the byte count.
+        Of an 8-bit record: the numbers the codes stand for, decoded where they arrive (upload8 leaves them as they are)."""
+        if self.shape8 is not None:
+            maps = self.upload8(names, device, chunk, workers, stats)
+            if torch.device(device).type != 'cuda':
+                return q8.dequantize_host(maps)
+            return _dequantizer(torch.device(device)).dequantize(*maps)
         if workers <= 0:
             workers = min(16, os.cpu_count() or 1)  # reader threads (a GPU box gives a job 16 CPUs)
         D, h, w = self.feature_shape(names[0])
@@ -197,6 +250,64 @@ class FeatureRecord:
         return out.permute(0, 2, 3, 1).contiguous() if pin else out
 
 
+    def upload8(self, names: Sequence[str], device, chunk: int = 256, workers: int = 0, stats: Optional[dict] = None) -> q8.Q8:
+        """Maps of `names` of an 8-bit record as pixel-major [N, h, w, D] codes and scales on the device: the pinned double
+        buffer of upload_pixel_major with a quarter of its bytes, and nothing to transpose.  Copies only are queued on the
+        CURRENT stream."""
+        if self.shape8 is None:
+            raise ValueError('%s is not held in 8 bits (records.quantize_record writes one that is)' % self.path)
+        if workers <= 0:
+            workers = min(16, os.cpu_count() or 1)
+        h, w, D = self.shape8
+        dev = torch.device(device)
+        pin = dev.type == 'cuda'
+        sizes = ((h, w, D), (h, w, q8.n_blocks(D)))
+        out = [torch.empty((len(names),) + s, dtype=torch.uint8, device=dev) for s in sizes]
+        n_stage = min(chunk, len(names))
+        stages = [[torch.empty((n_stage,) + s, dtype=torch.uint8, pin_memory=pin) for s in sizes] for _ in range(2 if len(names) > chunk else 1)]
+        free_ev = [None] * len(stages)
+        fds = [os.open(self.path, os.O_RDONLY) for _ in range(max(1, workers))]
+        t_decode = t_wait = 0.0
+        pool = ThreadPoolExecutor(max_workers=max(1, workers))
+        try:
+            for ci, s in enumerate(range(0, len(names), chunk)):
+                k, part = ci % len(stages), names[s:s + chunk]
+                t0 = time.perf_counter()
+                if free_ev[k] is not None:
+                    free_ev[k].synchronize()
+                t1 = time.perf_counter()
+                views = [v.numpy() for v in stages[k]]
+                list(pool.map(lambda j: self.read_feature8_into(part[j], views[0][j], views[1][j], fds[j % len(fds)]), range(len(part))))
+                t_wait, t_decode = t_wait + t1 - t0, t_decode + time.perf_counter() - t1
+                for o, v in zip(out, stages[k]):
+                    o[s:s + len(part)].copy_(v[:len(part)], non_blocking=pin)
+                if pin:
+                    free_ev[k] = torch.cuda.Event()
+                    free_ev[k].record(torch.cuda.current_stream(dev))
+        finally:
+            pool.shutdown()
+            for fd in fds:
+                os.close(fd)
+        if stats is not None:
+            stats.update(decode_s=stats.get('decode_s', 0.0) + t_decode, stage_wait_s=stats.get('stage_wait_s', 0.0) + t_wait,
+                         bytes=stats.get('bytes', 0) + sum(o.numel() for o in out))
+        return q8.Q8(out[0].view(torch.float8_e4m3fn), out[1].view(torch.float8_e8m0fnu))
+
+
+_dequantizers: dict = {}
+
+
+def _dequantizer(dev: torch.device):
+    """An engine for reading maps back where the caller has none (its maps' shape does not matter)."""
+    from .engine import PoseEngine
+    key = dev.index if dev.index is not None else torch.cuda.current_device()
+    if key not in _dequantizers:
+        before = torch.cuda.current_device()
+        _dequantizers[key] = PoseEngine(16, (16, 16), device=torch.device('cuda', key))
+        torch.cuda.set_device(before)
+    return _dequantizers[key]
+
+
 def write_feature_record(path: str, memory: Dict[str, np.ndarray], clutter: Dict[str, np.ndarray],
                          names: Dict[str, Sequence[str]], features: Dict[str, np.ndarray]) -> None:
     """Writes the ExtractFeatures.py format (:137-139,166-168,223); `features[name]` is [D, h, w]."""
@@ -209,6 +320,43 @@ def write_feature_record(path: str, memory: Dict[str, np.ndarray], clutter: Dict
         get[n] = np.asarray(f, dtype=np.float32)
     os.makedirs(os.path.dirname(os.path.abspath(path)), exist_ok=True)
     np.savez(path, **get)
+
+
+def write_feature_record8(path: str, memory: Dict[str, np.ndarray], clutter: Dict[str, np.ndarray],
+                          names: Dict[str, Sequence[str]], features: Dict[str, q8.Q8]) -> None:
+    """write_feature_record with maps held in 8 bits: `features[name]` is a pixel-major q8.Q8 [h, w, D] (PoseEngine.quantize or
+    q8.quantize_host), all of one shape.  Banks stay f32."""
+    get = {}
+    for st in memory:
+        get['memory_%s' % st] = np.asarray(memory[st], dtype=np.float32)
+        get['clutter_%s' % st] = np.asarray(clutter[st], dtype=np.float32)
+        get['names_%s' % st] = np.asarray(list(names[st]), dtype=str)
+    shape = None
+    for n, f in features.items():
+        if f.codes.dim() != 3 or tuple(f.codes.shape) != (shape or tuple(f.codes.shape)) or \
+                tuple(f.scale.shape) != tuple(f.codes.shape[:2]) + (q8.n_blocks(f.codes.shape[2]),):
+            raise ValueError('map %r: expected [h, w, D] of one shape, got %s' % (n, tuple(f.codes.shape)))
+        shape = tuple(f.codes.shape)
+        get[n] = np.concatenate([v.detach().cpu().contiguous().view(torch.uint8).numpy().reshape(-1) for v in f])
+    if shape is None:
+        raise ValueError('no feature maps')
+    get['features_8bit'] = np.asarray(shape, dtype=np.int64)
+    os.makedirs(os.path.dirname(os.path.abspath(path)), exist_ok=True)
+    np.savez(path, **get)
+
+
+def quantize_record(src: str, dst: str) -> int:
+    """Rewrites a feature record with its maps held in 8 bits (on the host; one image at a time, so that it needs room for the
+    8-bit maps only).  Returns the number of maps."""
+    if os.path.abspath(src) == os.path.abspath(dst):
+        raise ValueError('quantize_record: %s would overwrite its source' % dst)
+    with FeatureRecord(src) as rec:
+        if rec.shape8 is not None:
+            raise ValueError('%s is held in 8 bits already' % src)
+        maps = {n: q8.quantize_host(torch.from_numpy(rec.feature(n)).permute(1, 2, 0).contiguous()) for n in rec.image_keys}
+        write_feature_record8(dst, {s: rec.memory(s) for s in rec.subtypes}, {s: rec.clutter(s) for s in rec.subtypes},
+                              {s: rec.names(s) for s in rec.subtypes}, maps)
+    return len(maps)
 
 
 # ------------------------------------------------------------------ annotations

@@ -55,6 +55,9 @@ def build_parser():
     p.add_argument('--no_reload', action='store_true',
                    help='with --save_final_pred: solve every image again instead of keeping the entries the file already holds')
     p.add_argument('--accuracy_table', default='', type=str, help='directory of per-category records: print CalAccuracy table')
+    p.add_argument('--quantize_record', default='', type=str,
+                   help='write the category\'s feature record to this file with its maps held in 8 bits (a quarter of the bytes to read and '
+                        'upload; a run on that file solves on the numbers they stand for) and stop')
     p.add_argument('--batch', default=256, type=int, help='images per solve launch; the next batch is read and uploaded meanwhile')
     p.add_argument('--streams', default=2, type=int,
                    help='solver contexts, each on a stream of its own, taking the batches in turn: the next batch starts on the '
@@ -132,7 +135,8 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
 
     The images go through in batches (batch_plan): while earlier batches are solved, a helper thread reads the next one
     from the record into pinned memory and uploads it on a side stream (records.upload_pixel_major; DMA copies only,
-    the one transpose kernel of a batch runs when compute units are free).  Batches alternate between --streams solver
+    the one transpose kernel of a batch runs when compute units are free; records.upload8, and no kernel, from a record held
+    in 8 bits).  Batches alternate between --streams solver
     contexts, each with its own stream and workspaces: a solve is one workgroup per job for all its steps, so a launch
     ends with its slowest job while most compute units idle; the next batch's launches, queued on the other stream,
     take those units as they come free.  Batches do not change results (every job is independent)."""
@@ -162,7 +166,8 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
         slots.acquire()
         torch.cuda.set_device(dev)
         with torch.cuda.stream(side):
-            feats = rec.upload_pixel_major(names[lo:hi], dev, stats=stats)
+            upload = rec.upload8 if rec.shape8 is not None else rec.upload_pixel_major
+            feats = upload(names[lo:hi], dev, stats=stats)
             ready = torch.cuda.Event(enable_timing=timed)
             ready.record(side)
         if timed:
@@ -178,6 +183,8 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
             solver, clutter = build_solver(args, rec, subtypes, dev)
             solver.engine.reserve(biggest, int(solver.grid_theta.shape[1]))
             solver.prerender()
+            if rec.shape8 is not None and not solver.cfg.turn_off_clutter:
+                clutter = solver.clutter_banks8(clutter)
             ctxs.append((solver, clutter, torch.cuda.Stream(dev) if n_ctx > 1 else main))
         for st in ctxs:
             st[2].wait_stream(main)      # set-up (registration, pre-render) ran on the current stream
@@ -187,7 +194,8 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
             solver, clutter, stream = ctxs[bi % n_ctx]
             with torch.cuda.stream(stream):
                 stream.wait_event(ready)
-                feats.record_stream(stream)
+                for part in feats if isinstance(feats, tuple) else (feats,):
+                    part.record_stream(stream)
                 if timed:
                     b0 = torch.cuda.Event(enable_timing=True)
                     b0.record(stream)
@@ -270,6 +278,10 @@ def main(argv=None):
     if args.accuracy_table:
         _, text = records.accuracy_table_from_dir(args.accuracy_table, args.data_pendix)
         print(text)
+        return 0
+    if args.quantize_record:
+        n = records.quantize_record(record_path(args), args.quantize_record)
+        print('%d maps in 8 bits: %s' % (n, args.quantize_record))
         return 0
     world = int(os.environ.get('WORLD_SIZE', '1'))
     rank = int(os.environ.get('RANK', '0'))

@@ -352,6 +352,71 @@ def test_same_result_every_time(eng):
         assert torch.equal(eng.q8_clutter_score(a, b), first[0]) and torch.equal(eng.q8_product(a, b), first[1])
 
 
+# ------------------------------------------------------------------------------------------------ in the solver
+def test_solver_on_maps_in_8_bits():
+    """BatchPoseSolver on 8-bit maps is the solver on the numbers they stand for, bit for bit, with the 8-bit clutter scores."""
+    from nemo_amd.pose_solver import SolverConfig
+    from nemo_amd.workloads import twelve_class_workload
+    wl = twelve_class_workload(10, seed=5, cfg=SolverConfig(image_size=(256, 384), total_epochs=20), categories=['car', 'sofa', 'chair'])
+    s, eng = wl.solver, wl.solver.engine
+    maps = eng.quantize(wl.feats)
+    back = eng.dequantize(*maps)
+    # every number within half a step of its code: 2^-4 of it, or 2^-10 of the scale
+    step = torch.maximum(wl.feats.abs() * 2.0 ** -4, maps.scale.float() * 2.0 ** -10)
+    assert bool(((back - wl.feats).abs() <= step).all())
+    group = [int(m) for m in wl.mesh_idx]
+    rng = torch.Generator().manual_seed(1)
+    clutter = [torch.nn.functional.normalize(torch.randn(k, 128, generator=rng)).cuda() for k in (1, 7, 40)]
+    banks = s.clutter_banks8(clutter)
+    clu = s.clutter_scores_by_group(maps, group, banks)
+    assert torch.equal(clu, s.clutter_scores_by_group(maps, group, clutter))
+    for i, g in enumerate(group):                          # alone, each image against its own bank
+        one = q8.Q8(maps.codes[i:i + 1].contiguous(), maps.scale[i:i + 1].contiguous())
+        assert torch.equal(clu[i], eng.q8_clutter_score(one, eng.quantize(clutter[g]))[0])
+    a = s.solve_all(maps, None, wl.mesh_idx, clutter_scores=clu)
+    b = s.solve_all(back, None, wl.mesh_idx, clutter_scores=clu)
+    assert torch.equal(a.campos, b.campos) and torch.equal(a.loss, b.loss) and torch.equal(a.init_index, b.init_index)
+    c = s.solve_all(maps, wl.clutter, wl.mesh_idx)          # one clutter vector for all
+    d = s.solve_all(back, None, wl.mesh_idx, clutter_scores=eng.q8_clutter_score(maps, eng.quantize(wl.clutter)))
+    assert torch.equal(c.campos, d.campos) and torch.equal(c.loss, d.loss) and bool(torch.isfinite(c.loss).all())
+    with pytest.raises(ValueError, match='group_of_image'):
+        s.clutter_scores_by_group(maps, [0] * 9 + [3], banks)
+    with pytest.raises(ValueError, match='at least one clutter vector'):
+        s.clutter_banks8([clutter[0], clutter[1][:0]])
+
+
+def test_runner_on_a_record_in_8_bits(tmp_path):
+    """The file-driven runner on an 8-bit record: the solver on the record's numbers, in batches on two streams."""
+    from nemo_amd import mesh_utils, records, solve_all
+    from nemo_amd import synthetic as syn
+    rng = np.random.default_rng(3)
+    names, feats, mem, clu = {}, {}, {}, {}
+    for k, st in enumerate(('mesh01', 'mesh02')):
+        v, f = syn.class_mesh('car', 300 + 50 * k)
+        mesh_utils.save_off(str(tmp_path / ('%02d.off' % (k + 1))), v, f)
+        mem[st], clu[st] = syn.unit_rows(rng, len(v), 128), syn.unit_rows(rng, 6 + k, 128)
+        names[st] = ['%s_%d' % (st, i) for i in range(11)]
+        for n in names[st]:
+            feats[n] = syn.unit_rows(rng, 12 * 23, 128).reshape(12, 23, 128).transpose(2, 0, 1).copy()
+    src, dst = str(tmp_path / 'f32.npz'), str(tmp_path / 'q8.npz')
+    records.write_feature_record(src, mem, clu, names, feats)
+    records.quantize_record(src, dst)
+    args = solve_all.build_parser().parse_args(['--type_', 'car', '--record_file', dst, '--mesh_path', str(tmp_path), '--image_size', '96,184',
+                                                '--total_epochs', '15', '--batch', '8'])
+    with records.FeatureRecord(dst) as rec:
+        all_names, mesh_of = solve_all.category_jobs(rec, ['mesh01', 'mesh02'])
+        order = [i for pair in zip(range(11), range(11, 22)) for i in pair]   # the subtypes in turn
+        all_names, mesh_of = [all_names[i] for i in order], [mesh_of[i] for i in order]
+        got, _ = solve_all.solve_shard(args, rec, ['mesh01', 'mesh02'], all_names, mesh_of, 'cuda:0')
+        maps = rec.upload8(all_names, 'cuda:0', chunk=5)
+        assert torch.equal(rec.upload_pixel_major(all_names, 'cuda:0').cpu(),
+                           torch.stack([torch.from_numpy(rec.feature(n)).permute(1, 2, 0) for n in all_names]))
+        solver, clutter = solve_all.build_solver(args, rec, ['mesh01', 'mesh02'], 'cuda:0')
+        mesh = torch.tensor(mesh_of, dtype=torch.int32, device='cuda')
+        want = solver.solve_all(solver.engine.dequantize(*maps), None, mesh, clutter_scores=solver.clutter_scores_by_group(maps, mesh_of, clutter))
+    assert torch.equal(got[:, :8], want.packed())
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(eng):
     (a, _), (b, _) = rows8(12 * 23, 128, 91), rows8(8, 128, 92)

@@ -88,25 +88,34 @@ class FeatureRecord:
         """(byte offset of the array data in the .npz, shape) of a STORED little-endian f32 (8-bit record: u8) C-order member, else None
         (compressed record, other dtype: the caller falls back to the zipfile path)."""
         if not hasattr(self, '_zinfo'):
+            self._layouts, self._headers = {}, {}
+            self._fd = os.open(self.path, os.O_RDONLY)
             with zipfile.ZipFile(self.path) as zf:
-                self._zinfo = {i.filename: i for i in zf.infolist()}
-            self._layouts = {}
+                self._zinfo = {i.filename: i for i in zf.infolist()}   # last: its presence says that the rest is there
         if name in self._layouts:
             return self._layouts[name]
         info = self._zinfo.get(name + '.npy')
         lay = None
         if info is not None and info.compress_type == zipfile.ZIP_STORED:
-            with open(self.path, 'rb') as fh:
-                fh.seek(info.header_offset)
-                local = fh.read(30)
-                n_name, n_extra = struct.unpack('<HH', local[26:30])
-                start = info.header_offset + 30 + n_name + n_extra
-                fh.seek(start)
-                version = np.lib.format.read_magic(fh)
-                shape, fortran, dtype = (np.lib.format.read_array_header_1_0(fh) if version == (1, 0)
-                                         else np.lib.format.read_array_header_2_0(fh))
-                if dtype == np.dtype('u1' if self.shape8 is not None else '<f4') and not fortran:
-                    lay = (fh.tell(), tuple(shape))
+            # zip header (30 bytes, then the two lengths given in it), npy magic (8) and length, npy header: of maps of one shape the
+            # latter are the same bytes, parsed once
+            block = os.pread(self._fd, 1024, info.header_offset)
+            start = 30 + sum(struct.unpack('<HH', block[26:30]))
+            head = block[start:start + 10 + struct.unpack('<H', block[start + 8:start + 10])[0]] if len(block) >= start + 10 else b''
+            if head not in self._headers:
+                with open(self.path, 'rb') as fh:
+                    fh.seek(info.header_offset + start)
+                    version = np.lib.format.read_magic(fh)
+                    shape, fortran, dtype = (np.lib.format.read_array_header_1_0(fh) if version == (1, 0)
+                                             else np.lib.format.read_array_header_2_0(fh))
+                    good = dtype == np.dtype('u1' if self.shape8 is not None else '<f4') and not fortran
+                    known = (fh.tell() - info.header_offset - start, tuple(shape)) if good else None
+                    if version == (1, 0) and start + len(head) <= len(block):
+                        self._headers[head] = known
+            else:
+                known = self._headers[head]
+            if known is not None:
+                lay = (info.header_offset + start + known[0], known[1])
         self._layouts[name] = lay
         return lay
 
@@ -151,7 +160,7 @@ class FeatureRecord:
             done += n
 
     def read_feature8_into(self, name: str, codes: np.ndarray, scale: np.ndarray, fd: int) -> None:
-        """Fill `codes` (u8, h w D bytes) and `scale` (u8) with the map `name` of an 8-bit record: two preads, or the zip reader
+        """Fill `codes` (u8, h w D bytes) and `scale` (u8) with the map `name` of an 8-bit record: one read, or the zip reader
         where the record is compressed."""
         lay = self._layout(name)
         if lay is None:
@@ -160,10 +169,12 @@ class FeatureRecord:
             scale.reshape(-1)[:] = f.scale.view(torch.uint8).numpy().reshape(-1)
             return
         off, shape = lay
-        if shape != (codes.size + scale.size,):
-            raise ValueError('feature map %r has shape %s, expected %d bytes' % (name, shape, codes.size + scale.size))
-        self._pread(fd, name, codes, off)
-        self._pread(fd, name, scale, off + codes.size)
+        size = codes.size + scale.size
+        if shape != (size,):
+            raise ValueError('feature map %r has shape %s, expected %d bytes' % (name, shape, size))
+        if os.preadv(fd, [codes.reshape(-1), scale.reshape(-1)], off) != size:   # cut short: by parts
+            self._pread(fd, name, codes, off)
+            self._pread(fd, name, scale, off + codes.size)
 
     def feature_shape(self, name: str):
         """(D, h, w)"""
@@ -175,6 +186,9 @@ class FeatureRecord:
 
     def close(self):
         self._z.close()
+        if getattr(self, '_fd', None) is not None:
+            os.close(self._fd)
+            self._fd = None
 
     def __enter__(self):
         return self
@@ -250,7 +264,7 @@ class FeatureRecord:
         return out.permute(0, 2, 3, 1).contiguous() if pin else out
 
 
-    def upload8(self, names: Sequence[str], device, chunk: int = 256, workers: int = 0, stats: Optional[dict] = None) -> q8.Q8:
+    def upload8(self, names: Sequence[str], device, chunk: int = 64, workers: int = 0, stats: Optional[dict] = None) -> q8.Q8:
         """Maps of `names` of an 8-bit record as pixel-major [N, h, w, D] codes and scales on the device: the pinned double
         buffer of upload_pixel_major with a quarter of its bytes, and nothing to transpose.  Copies only are queued on the
         CURRENT stream."""
@@ -259,6 +273,7 @@ class FeatureRecord:
         if workers <= 0:
             workers = min(16, os.cpu_count() or 1)
         h, w, D = self.shape8
+        self._layout(names[0])   # the record's directory, before the threads ask for it
         dev = torch.device(device)
         pin = dev.type == 'cuda'
         sizes = ((h, w, D), (h, w, q8.n_blocks(D)))

@@ -699,11 +699,10 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
 }
 
 // Long rows (K > 256): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS.  There is
-// one buffer: the three workgroups of a compute unit fill each other's waits, which measured better than two buffers and two workgroups
-// (more rows of a on their way at a time).  A step is 32 matrix instructions a wave (1024 cycles) against 128 widening ones and 16 KB out
-// of LDS; the block is multiplied in halves to keep the registers for three.
+// one buffer: a wave reads its 16 KB of a step into registers, and once all waves have, the next step is copied under the widening (128
+// instructions a wave) and the products (32, 1024 cycles).
 template <class TT>
-__global__ __launch_bounds__(256, 3) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
+__global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
   __shared__ __align__(16) uint8_t codes[2][128 * Q8_BLOCK];  // a, b
   __shared__ float scale[2][128];
   // the column tiles of the same rows follow each other on one XCD, whose L2 keeps the rows of a
@@ -714,55 +713,66 @@ __global__ __launch_bounds__(256, 3) void q8_product_long_kernel(Q8Args A, int t
   const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cols = min(S.n1 - S.n0, A.n_cols), n0 = (int)(id % cuts) * 128, m1 = S.r1;
   if (n0 >= cols) return;
-  const uint8_t *pa[4], *pb[4];  // the thread's 16-byte pieces of a step, 32 rows apart
+  // the thread's 16-byte pieces of a step, 32 rows apart: where their rows begin behind the tile's first (128 rows: 32 bits)
+  const uint8_t *ta = A.a + (size_t)S.r0 * A.K, *tb = A.b + ((size_t)S.n0 + n0) * A.K;
+  uint32_t pa[4], pb[4];
   int r0, q;
   q8_at<1>(tid, r0, q);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    pa[j] = A.a + (size_t)min(S.r0 + r0 + 32 * j, m1 - 1) * A.K;
-    pb[j] = A.b + ((size_t)S.n0 + min(n0 + r0 + 32 * j, cols - 1)) * A.K;
+    pa[j] = (uint32_t)min(r0 + 32 * j, m1 - 1 - S.r0) * (uint32_t)A.K;
+    pb[j] = (uint32_t)min(r0 + 32 * j, cols - 1 - n0) * (uint32_t)A.K;
   }
   const uint8_t *pe = tid < 128 ? A.ae + (size_t)min(S.r0 + tid, m1 - 1) * A.nb : A.be + ((size_t)S.n0 + min(n0 + tid - 128, cols - 1)) * A.nb;
+  uint32_t e;
+  auto copy = [&](int b) {
+    const uint32_t k = (uint32_t)min(b * Q8_BLOCK + 16 * q, A.K - 16);  // past the end of a row: its last piece, taken for zeros below
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      q8_copy16(ta + (pa[j] + k), &codes[0][4096 * j + 1024 * w]);
+      q8_copy16(tb + (pb[j] + k), &codes[1][4096 * j + 1024 * w]);
+    }
+    e = pe[b];
+  };
   const int mw = 64 * (w >> 1), nw = 64 * (w & 1);  // the wave's corner of the tile
   f16v acc[2][2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int t = 0; t < 2; ++t) acc[s][t] = q8_zero();
+  copy(0);
   for (int b = 0; b < A.nb; ++b) {
-    const int k = min(b * Q8_BLOCK + 16 * q, A.K - 16);  // past the end of a row: its last piece, taken for zeros below
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      q8_copy16(pa[j] + k, &codes[0][4096 * j + 1024 * w]);
-      q8_copy16(pb[j] + k, &codes[1][4096 * j + 1024 * w]);
-    }
-    scale[tid >> 7][tid & 127] = q8_scale(pe[b]);
+    scale[tid >> 7][tid & 127] = q8_scale(e);
     q8_wait_copies();
     __syncthreads();
     const int left = A.K - b * Q8_BLOCK;
-    const float s0 = scale[0][mw + i], s1 = scale[0][mw + 32 + i], t0 = scale[1][nw + 2 * i], t1 = scale[1][nw + 2 * i + 1];
-    auto get = [&](int which, int row, int u, float s, bf8v (&v)[2]) {
-      u4va x = *(const u4va *)&codes[which][q8_place<1>(row, 2 * u + h)];
-      if (left < Q8_BLOCK && 16 * (2 * u + h) >= left) x = u4va{0, 0, 0, 0};
-      v[0] = q8_numbers(x[0], x[1], s);
-      v[1] = q8_numbers(x[2], x[3], s);
-    };
+    const float sx[2] = {scale[0][mw + i], scale[0][mw + 32 + i]}, sy[2] = {scale[1][nw + 2 * i], scale[1][nw + 2 * i + 1]};
+    Q8Raw x[2], y[2];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      bf8v x0[2], x1[2], y0[2], y1[2];
-      get(0, mw + i, u, s0, x0);
-      get(1, nw + 2 * i, u, t0, y0);
-      get(0, mw + 32 + i, u, s1, x1);
-      get(1, nw + 2 * i + 1, u, t1, y1);
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0[e], y0[e], acc[0][0], 0, 0, 0);
-        acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1[e], y0[e], acc[1][0], 0, 0, 0);
-        acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0[e], y1[e], acc[0][1], 0, 0, 0);
-        acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1[e], y1[e], acc[1][1], 0, 0, 0);
+      for (int u = 0; u < 4; ++u) {
+        x[s].v[u] = *(const u4va *)&codes[0][q8_place<1>(mw + 32 * s + i, 2 * u + h)];
+        y[s].v[u] = *(const u4va *)&codes[1][q8_place<1>(nw + 2 * i + s, 2 * u + h)];
       }
+    __syncthreads();  // the buffer has been read
+    if (b + 1 < A.nb) copy(b + 1);
+    if (left < Q8_BLOCK) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (16 * (2 * u + h) >= left) x[0].v[u] = x[1].v[u] = y[0].v[u] = y[1].v[u] = u4va{0, 0, 0, 0};
     }
-    __syncthreads();  // nobody reads the buffer any more
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const bf8v x0 = q8_numbers(x[0].v[u][2 * g], x[0].v[u][2 * g + 1], sx[0]), y0 = q8_numbers(y[0].v[u][2 * g], y[0].v[u][2 * g + 1], sy[0]);
+        acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0, y0, acc[0][0], 0, 0, 0);
+        const bf8v x1 = q8_numbers(x[1].v[u][2 * g], x[1].v[u][2 * g + 1], sx[1]), y1 = q8_numbers(y[1].v[u][2 * g], y[1].v[u][2 * g + 1], sy[1]);
+        acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1, y0, acc[1][0], 0, 0, 0);
+        acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0, y1, acc[0][1], 0, 0, 0);
+        acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1, y1, acc[1][1], 0, 0, 0);
+      }
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s)

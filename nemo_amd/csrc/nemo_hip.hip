@@ -1259,10 +1259,12 @@ static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, vo
   const hipStream_t st = (hipStream_t)stream;
   typename TT::T *out = (typename TT::T *)d_out;
   const size_t chunks = ((size_t)A.n_cols + 127) / 128, cus = (size_t)ctx->n_cu;
-  // Short rows: 8 waves over 512 / nb columns, or 8 / wc of them to the same columns where there are fewer.  As many rows to a workgroup, up to
-  // 128 (f32) or 256 (bf16: the same bytes of results), as still give 2 workgroups to a compute unit.
+  // Short rows: 8 waves over 512 / nb columns of a bf16 result (wc = 8), over half of them in f32, two to the same columns: 1 KB of a row
+  // either way.  (262144 rows x 1095 x 128, whose rows begin anywhere in a line: f32 315 us with wc = 8, 233 with 4; bf16 192 and 188, but
+  // 135 and 161 where rows are whole lines.)  Fewer where there are fewer columns.  As many rows to a workgroup, up to 128 (f32) or 256, as
+  // still give 2 workgroups to a compute unit.
   const int per_wave = A.nb == 1 ? 64 : 32;
-  int wc = 8;
+  int wc = sizeof(typename TT::T) == 4 ? 4 : 8;
   while (wc > 1 && A.n_cols <= per_wave * (wc / 2)) wc /= 2;
   const size_t cuts = ((size_t)A.n_cols + per_wave * wc - 1) / ((size_t)per_wave * wc);
   int rt = (sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR) / 32;

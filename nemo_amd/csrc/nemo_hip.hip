@@ -1345,12 +1345,13 @@ int nemo_q8_clutter_score(nemo_ctx *ctx, const uint8_t *d_feat, const uint8_t *d
   A.seg_rows = hw;
   A.n_seg = n_img; A.n_banks = n_banks;
   A.bank_off = d_bank_off; A.bank_of = d_bank_of;
-  // The largest tile of pixels per workgroup that still gives every compute unit a workgroup; where not even 256 pixels do, 32 with
-  // the bank dealt to the waves.
+  // The largest tile of pixels per workgroup that still gives every compute unit a workgroup, 256 pixels from half of them on; below that,
+  // 32 pixels with the bank dealt to the waves (D = 128, K = 2560, maps of 80 x 100: one map 13 us that way and 35 with 256 pixels,
+  // four maps 41 and 35).
   const auto tiles = [&](size_t tm) { return (size_t)n_img * (((size_t)hw + tm - 1) / tm); };
   const size_t cus = (size_t)ctx->n_cu;
   const bool wide = ctx->cfg.feat_dim == 256;
-  const int T = !wide && tiles(1024) >= cus ? 4 : tiles(512) >= cus ? 2 : tiles(256) >= cus ? 1 : 0;
+  const int T = !wide && tiles(1024) >= cus ? 4 : tiles(512) >= cus ? 2 : 2 * tiles(256) >= cus ? 1 : 0;
   const size_t blocks = tiles(T ? 256 * T : 32);
   if (blocks > (1u << 23) - 1) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_q8_clutter_score: too many pixels for one launch");
   DeviceGuard on(ctx->device);

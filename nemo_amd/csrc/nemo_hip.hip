@@ -1259,35 +1259,36 @@ static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, vo
   const hipStream_t st = (hipStream_t)stream;
   typename TT::T *out = (typename TT::T *)d_out;
   const size_t chunks = ((size_t)A.n_cols + 127) / 128, cus = (size_t)ctx->n_cu;
-  // Short rows: 8 waves over 512 / nb columns of a bf16 result (wc = 8), over half of them in f32, two to the same columns: 1 KB of a row
-  // either way.  (262144 rows x 1095 x 128, whose rows begin anywhere in a line: f32 315 us with wc = 8, 233 with 4; bf16 192 and 188, but
-  // 135 and 161 where rows are whole lines.)  Fewer where there are fewer columns.  As many rows to a workgroup, up to 128 (f32) or 256, as
-  // still give 2 workgroups to a compute unit.
-  const int per_wave = A.nb == 1 ? 64 : 32;
-  int wc = sizeof(typename TT::T) == 4 ? 4 : 8;
-  while (wc > 1 && A.n_cols <= per_wave * (wc / 2)) wc /= 2;
-  const size_t cuts = ((size_t)A.n_cols + per_wave * wc - 1) / ((size_t)per_wave * wc);
-  int rt = (sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR) / 32;
-  while (rt > 8 / wc && rt > 1 && q8_tiles(A, 32 * rt) * cuts < 2 * cus) rt /= 2;
-  const size_t tiles = q8_tiles(A, 32 * rt);
-  if (A.nb <= 2 && (size_t)A.M >= 64 * (size_t)A.n_seg && tiles * cuts >= cus / 4) {
-    const size_t blocks = (tiles * cuts + 7) / 8 * 8;
+  // Up to 32 columns, or so few rows that 32 x 128 products a workgroup make at most 3 workgroups for 2 compute units, or fewer than 64 rows a
+  // segment: one wave for 32 x 32 (f32 results: 1000 x 1000 x 128 4.3 us that way, 5.9 and 5.7 with the kernels below; 300 x 8000 x 128
+  // 7.1, 6.5 and 6.1; 262144 x 16 x 128 11.5, 21.5 and 20.7).
+  if (A.n_cols <= 32 || 2 * q8_tiles(A, 32) * chunks <= 3 * cus || (size_t)A.M < 64 * (size_t)A.n_seg) {
+    const bool split = A.nb > 2;
+    const int across = A.n_cols <= 32 ? 1 : 4;
+    const size_t few = q8_tiles(A, split ? 32 : 128 / across), cols = split ? ((size_t)A.n_cols + 31) / 32 : across == 1 ? 1 : chunks;
+    if (few > Q8_MAX_BLOCKS || cols > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
+    const dim3 grid((unsigned)few, (unsigned)cols);
+    if (split) hipLaunchKernelGGL((q8_product_few_kernel<TT, 4>), grid, dim3(256), 0, st, A, across, out);
+    else hipLaunchKernelGGL((q8_product_few_kernel<TT, 1>), grid, dim3(256), 0, st, A, across, out);
+  } else if (A.nb == 1) {
+    // Short rows: 8 waves over 512 columns of a bf16 result (wc = 8), over half of them in f32, two to the same columns: 1 KB of a row
+    // either way.  (262144 rows x 1095 x 128, whose rows begin anywhere in a line: f32 315 us with wc = 8, 233 with 4; bf16 192 and 188, but
+    // 135 and 161 where rows are whole lines.)  Fewer where there are fewer columns.  As many rows to a workgroup, up to 128 (f32) or 256,
+    // as still give 2 workgroups to a compute unit.
+    int wc = sizeof(typename TT::T) == 4 ? 4 : 8;
+    while (wc > 1 && A.n_cols <= 64 * (wc / 2)) wc /= 2;
+    const size_t cuts = ((size_t)A.n_cols + 64 * wc - 1) / ((size_t)64 * wc);
+    int rt = (sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR) / 32;
+    while (rt > 8 / wc && rt > 1 && q8_tiles(A, 32 * rt) * cuts < 2 * cus) rt /= 2;
+    const size_t tiles = q8_tiles(A, 32 * rt), blocks = (tiles * cuts + 7) / 8 * 8;
     if (blocks > (1u << 23) - 1) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
     const dim3 grid((unsigned)blocks), wg(512);
-    const int n = (int)tiles, c = (int)cuts;
-    if (A.nb == 1 && A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, false>), grid, wg, 0, st, A, n, c, wc, rt, out);
-    else if (A.nb == 1) hipLaunchKernelGGL((q8_product_short_kernel<TT, 1, true>), grid, wg, 0, st, A, n, c, wc, rt, out);
-    else if (A.K == 256) hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, false>), grid, wg, 0, st, A, n, c, wc, rt, out);
-    else hipLaunchKernelGGL((q8_product_short_kernel<TT, 2, true>), grid, wg, 0, st, A, n, c, wc, rt, out);
-  } else if (A.nb > 2 && (size_t)A.M >= 64 * (size_t)A.n_seg && q8_tiles(A, 128) * chunks >= cus / 4) {
-    // Long rows: tiles of 128 x 128, from as many on as occupy a quarter of the compute units.
+    if (A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, false>), grid, wg, 0, st, A, (int)tiles, (int)cuts, wc, rt, out);
+    else hipLaunchKernelGGL((q8_product_short_kernel<TT, true>), grid, wg, 0, st, A, (int)tiles, (int)cuts, wc, rt, out);
+  } else {
     const size_t n = q8_tiles(A, 128), blocks = (n * chunks + 7) / 8 * 8;
     if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
     hipLaunchKernelGGL((q8_product_long_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, st, A, (int)n, (int)chunks, out);
-  } else {
-    const size_t few = q8_tiles(A, 32);
-    if (few > Q8_MAX_BLOCKS || chunks > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
-    hipLaunchKernelGGL((q8_product_few_kernel<TT>), dim3((unsigned)few, (unsigned)chunks), dim3(256), 0, st, A, out);
   }
   HIP_TRY(ctx, hipGetLastError());
   return NEMO_OK;

@@ -435,7 +435,7 @@ __device__ __forceinline__ bool q8_find(const Q8Args &A, unsigned work, int TM, 
 
 // Operands of v_mfma_f32_32x32x16_bf16: lane l holds row l % 32 and, of a block of 128 channels, the 16-byte chunks 2 u + l / 32, u = 0 .. 3.
 // A chunk feeds two instructions, eight channels each; which channels meet in which instruction does not matter as long as it is the
-// same for both operands (and it is the same in every kernel here, so a product has the same bits whichever computes it).
+// same for both operands (and it is the same in every kernel here: a product of up to 256 channels has the same bits whichever computes it).
 __device__ __forceinline__ bf8v q8_numbers(uint32_t lo, uint32_t hi, float s) {
   const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, true);
   const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, true);
@@ -519,31 +519,79 @@ __device__ __forceinline__ void q8_store(typename TT::T *out, int ld, int m0, in
   }
 }
 
-// Few rows: a wave owns 32 rows x 32 columns, a workgroup 4 such tiles side by side; operands come straight from memory, a block of 128
-// channels ahead.  Any K.
-template <class TT>
-__global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, typename TT::T *__restrict__ out) {
+// Few rows, or few columns: a wave owns 32 x 32 products.  Its 4 KB of either operand and block are read in order of addresses, a block
+// ahead, and turned in LDS of its own (read by rows, a load instruction touches 32 lines for 32 bytes of each: 16 blocks of one tile took
+// 18 us that way).  KS = 1: `across` of the 4 waves of a workgroup stand side by side, the others below them.  KS = 4, for long rows: they deal the blocks of the same tile
+// among them, and their sums are added in the order of the waves.
+template <class TT, int KS>
+__global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, int across, typename TT::T *__restrict__ out) {
+  __shared__ __align__(16) uint8_t turn[4][2][4096];
   Q8Seg S;
-  if (!q8_find<4>(A, blockIdx.x, 32, S)) return;
-  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+  if (!q8_find<4>(A, blockIdx.x, KS == 1 ? 128 / across : 32, S)) return;
+  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int cols = min(S.n1 - S.n0, A.n_cols);
-  const int n0 = ((int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)) * 32;
-  if (n0 >= cols) return;
-  const size_t ra = (size_t)min(S.r0 + i, S.r1 - 1), rb = (size_t)S.n0 + min(n0 + i, cols - 1);
-  f16v acc = q8_zero();
-  Q8Raw xa = q8_load(A.a + ra * A.K, 0, h, A.K), xb = q8_load(A.b + rb * A.K, 0, h, A.K);
-  uint32_t ea = A.ae[ra * A.nb], eb = A.be[rb * A.nb];
-  for (int b = 0; b < A.nb; ++b) {
-    const Q8Frag fa = q8_frag(xa, q8_scale(ea)), fb = q8_frag(xb, q8_scale(eb));
-    if (b + 1 < A.nb) {
-      xa = q8_load(A.a + ra * A.K, b + 1, h, A.K);
-      xb = q8_load(A.b + rb * A.K, b + 1, h, A.K);
-      ea = A.ae[ra * A.nb + b + 1];
-      eb = A.be[rb * A.nb + b + 1];
-    }
-    acc = q8_mfma(fa, fb, acc);
+  const int n0 = (KS == 1 ? (int)blockIdx.y * across + w % across : (int)blockIdx.y) * 32;
+  if (KS == 1) S.r0 += 32 * (w / across);
+  if (n0 >= cols || S.r0 >= S.r1) return;
+  const uint8_t *pa[4], *pb[4];  // the lane's 16-byte pieces of a block
+  int at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    int row;
+    q8_at<1>(64 * j + lane, row, at[j]);
+    at[j] *= 16;
+    pa[j] = A.a + (size_t)min(S.r0 + row, S.r1 - 1) * A.K + at[j];
+    pb[j] = A.b + ((size_t)S.n0 + min(n0 + row, cols - 1)) * A.K + at[j];
   }
-  q8_store<TT>(out, A.n_cols, S.r0, S.r1, n0, cols, i, h, acc);
+  const uint8_t *ea = A.ae + (size_t)min(S.r0 + i, S.r1 - 1) * A.nb, *eb = A.be + ((size_t)S.n0 + min(n0 + i, cols - 1)) * A.nb;
+  u4va ga[4], gb[4];
+  uint32_t sa = 0, sb = 0;
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = b * Q8_BLOCK + at[j] < A.K;
+      ga[j] = in ? *(const u4va *)(pa[j] + b * Q8_BLOCK) : u4va{0, 0, 0, 0};
+      gb[j] = in ? *(const u4va *)(pb[j] + b * Q8_BLOCK) : u4va{0, 0, 0, 0};
+    }
+    sa = ea[b];
+    sb = eb[b];
+  };
+  f16v acc = q8_zero();
+  int b = KS == 1 ? 0 : w;
+  if (b < A.nb) fetch(b);
+  for (; b < A.nb; b += KS) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      *(u4va *)&turn[w][0][16 * (64 * j + lane)] = ga[j];
+      *(u4va *)&turn[w][1][16 * (64 * j + lane)] = gb[j];
+    }
+    const float fa = q8_scale(sa), fb = q8_scale(sb);
+    q8_wave_sync();
+    Q8Raw x, y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      x.v[u] = *(const u4va *)&turn[w][0][q8_place<1>(i, 2 * u + h)];
+      y.v[u] = *(const u4va *)&turn[w][1][q8_place<1>(i, 2 * u + h)];
+    }
+    if (b + KS < A.nb) fetch(b + KS);
+    acc = q8_mfma(q8_frag(x, fa), q8_frag(y, fb), acc);
+    q8_wave_sync();
+  }
+  if (KS == 1) {
+    q8_store<TT>(out, A.n_cols, S.r0, S.r1, n0, cols, i, h, acc);
+    return;
+  }
+  float *part = (float *)&turn[0][0][0];  // 4 KB of the wave's own 8
+#pragma unroll
+  for (int r = 0; r < 16; ++r) part[w * 2048 + r * 64 + lane] = acc[r];
+  __syncthreads();
+  if (n0 + i >= cols) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {  // wave w adds and stores rows 8 w .. 8 w + 7 of the tile
+    const int at = (4 * w + k) * 64 + lane, m = S.r0 + 8 * w + 4 * h + k;
+    const float sum = ((part[at] + part[2048 + at]) + part[2 * 2048 + at]) + part[3 * 2048 + at];
+    if (m < S.r1) out[(size_t)m * A.n_cols + n0 + i] = TT::put(sum);
+  }
 }
 
 // The bank's way to LDS, for the kernels that keep their rows of a in registers (8 waves, K <= 128 NB): SR rows at a time as codes, copied
@@ -599,15 +647,20 @@ template <class TT, int NT>
 __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int m0, int m1, int n0, int n1, int i, int h, const f16v (&acc)[NT]) {
   typedef typename TT::T T;
   const uint32_t at = (uint32_t)(4 * h * ld + NT * i) * (uint32_t)sizeof(T);
-  char *base = (char *)(out + (size_t)m0 * ld + n0);
-  auto to = [&](int r) { return base + (size_t)(8 * (r >> 2) + (r & 3)) * ld * sizeof(T) + at; };
+  T *base = out + (size_t)m0 * ld + n0;
   if (m0 + 32 <= m1 && n0 + 32 * NT <= n1) {
+    // A row's address stays a scalar and the lane's place 32 bits, so that the store instruction adds them (the empty asm keeps the compiler
+    // from summing them in vector registers, an instruction and two registers a store).
+    uint32_t place = at;
+    asm("" : "+v"(place));
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       Q8Out<TT, NT> o;
 #pragma unroll
       for (int t = 0; t < NT; ++t) o.v[t] = TT::put(acc[t][r]);
-      *(Q8Out<TT, NT> *)to(r) = o;
+      uintptr_t row = (uintptr_t)(base + (size_t)(8 * (r >> 2) + (r & 3)) * ld);
+      asm("" : "+s"(row));
+      __builtin_memcpy((char GAS *)row + place, &o, sizeof(o));
     }
   } else {
 #pragma unroll
@@ -615,20 +668,20 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
       if (n0 + NT * i + t >= n1) break;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (m0 + 8 * (r >> 2) + (r & 3) + 4 * h < m1) ((T *)to(r))[t] = TT::put(acc[t][r]);
+        if (m0 + 8 * (r >> 2) + (r & 3) + 4 * h < m1) ((T *)((char *)(base + (size_t)(8 * (r >> 2) + (r & 3)) * ld) + at))[t] = TT::put(acc[t][r]);
     }
   }
 }
-// Short rows (K <= 256).  What bounds these products is the result's way to memory (a row of 128 channels meets a row of the bank in 256
+
+// Short rows (K <= 128).  What bounds these products is the result's way to memory (a row of 128 channels meets a row of the bank in 256
 // operations, but leaves 4 bytes), so the work is cut for the stores: the 8 waves of a workgroup own neighbouring columns of the same
-// rows, 32 NT each, whose bank rows stay in registers, and the rows pass by, up to 256 of them copied to LDS as codes before the
-// first product.  A workgroup then writes 512 / NB columns of 32 rows at about the same time, which fills whole lines also where out's rows
-// begin in the middle of one, and waits for no store.  Where the bank has fewer columns, 8 / wc waves share them and take the row tiles in
-// turn.
+// rows, 64 each, whose bank rows stay in registers, and the rows pass by, up to 256 of them copied to LDS as codes before the
+// first product.  A workgroup then writes 512 columns of 32 rows at about the same time, which fills whole lines also where out's rows
+// begin in the middle of one, and waits for no store.  With wc < 8, 8 / wc waves share the columns and take the row tiles in turn.
 constexpr int Q8_PR = 256;  // rows per workgroup, at most
-template <class TT, int NB, bool TAIL>
+template <class TT, bool TAIL>
 __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int tiles, int cuts, int wc, int rt, typename TT::T *__restrict__ out) {
-  constexpr int NT = 2 / NB;
+  constexpr int NB = 1, NT = 2;
   typedef Q8Bank<NB, TAIL, sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR, 1> Rows;
   __shared__ __align__(16) Rows L;
   __shared__ __align__(16) uint8_t turn[8][4096];
@@ -698,7 +751,7 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
   }
 }
 
-// Long rows (K > 256): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS.  There is
+// Long rows (K > 128): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS.  There is
 // one buffer: a wave reads its 16 KB of a step into registers, and once all waves have, the next step is copied under the widening (128
 // instructions a wave) and the products (32, 1024 cycles).
 template <class TT>

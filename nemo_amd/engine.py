@@ -343,6 +343,7 @@ class PoseEngine:
         n, image, c = room[0], room[1:-1], room[-1]
         slot_at = None
         if slots is not None:
+            self._ready(slots, torch.int32, 'slots')
             n = slots.shape[0] if slots.dim() else 0
             slot_at = self._index(slots, 'slots', n, room[0])
         shape = (n, c) + image if channel_major else (n,) + image + (c,)

@@ -101,7 +101,8 @@ class FeatureRecord:
             # latter are the same bytes, parsed once
             block = os.pread(self._fd, 1024, info.header_offset)
             start = 30 + sum(struct.unpack('<HH', block[26:30]))
-            head = block[start:start + 10 + struct.unpack('<H', block[start + 8:start + 10])[0]] if len(block) >= start + 10 else b''
+            end = start + 10 + struct.unpack('<H', block[start + 8:start + 10])[0] if len(block) >= start + 10 else len(block) + 1
+            head = block[start:end] if end <= len(block) else b''
             if head not in self._headers:
                 with open(self.path, 'rb') as fh:
                     fh.seek(info.header_offset + start)
@@ -110,7 +111,7 @@ class FeatureRecord:
                                              else np.lib.format.read_array_header_2_0(fh))
                     good = dtype == np.dtype('u1' if self.shape8 is not None else '<f4') and not fortran
                     known = (fh.tell() - info.header_offset - start, tuple(shape)) if good else None
-                    if version == (1, 0) and start + len(head) <= len(block):
+                    if version == (1, 0) and head:
                         self._headers[head] = known
             else:
                 known = self._headers[head]
@@ -186,9 +187,15 @@ class FeatureRecord:
 
     def close(self):
         self._z.close()
-        if getattr(self, '_fd', None) is not None:
+        self._forget()
+
+    def _forget(self):
+        if hasattr(self, '_zinfo'):
+            del self._zinfo      # asked for a layout again, the record opens its file again
             os.close(self._fd)
-            self._fd = None
+
+    def __del__(self):
+        self._forget()
 
     def __enter__(self):
         return self

@@ -280,6 +280,8 @@ def main(argv=None):
         print(text)
         return 0
     if args.quantize_record:
+        if int(os.environ.get('RANK', '0')) != 0:   # one writer
+            return 0
         n = records.quantize_record(record_path(args), args.quantize_record)
         print('%d maps in 8 bits: %s' % (n, args.quantize_record))
         return 0

@@ -125,3 +125,29 @@ def test_runner_writes_a_record_in_8_bits(tmp_path, capsys):
     assert '7 maps in 8 bits' in capsys.readouterr().out
     with records.FeatureRecord(dst) as r:
         assert r.shape8 == (5, 9, 128)
+
+
+def test_record_used_again_after_close_and_with_long_names(tmp_path):
+    """Layouts are found again after close(), for members with other headers and for names longer than what is read of a header at once."""
+    from nemo_amd import records
+    long = 'x' * 2000
+    path = str(tmp_path / 'r.npz')
+    a, b, c = (np.arange(n * 20, dtype=np.float32).reshape(n, 4, 5) for n in (3, 30, 300))
+    np.savez(path, **{'a': a, 'b': b, 'c': c, long: 2 * a, long + 'y': 3 * b, 'f16': a.astype(np.float16), 'fortran': np.asfortranarray(b)})
+    r = records.FeatureRecord(path)
+    for _ in range(2):
+        for name, want in (('a', a), (long, 2 * a), ('b', b), (long + 'y', 3 * b), ('c', c), ('a', a)):
+            into = np.empty_like(want)
+            r.read_feature_into(name, into)
+            assert np.array_equal(into, want) and r._layout(name)[1] == want.shape
+        assert r._layout('f16') is None and r._layout('fortran') is None
+        r.close()
+
+
+def test_runner_writes_the_record_once(tmp_path, monkeypatch):
+    from nemo_amd import solve_all
+    src, _, _ = _record(tmp_path, n=2)
+    dst = tmp_path / 'q8.npz'
+    monkeypatch.setenv('RANK', '1')
+    assert solve_all.main(['--type_', 'car', '--record_file', src, '--quantize_record', str(dst)]) == 0
+    assert not dst.exists()

@@ -179,6 +179,23 @@ def test_scales_of_any_size_meet_exactly(eng):
     close(eng.q8_product(a, b), a64 * 2.0 ** -100, b64 * 2.0 ** 100, 128)
 
 
+@pytest.mark.parametrize('k', [128, 256, 1024])
+def test_scale_bytes_at_the_ends_in_products(eng, k):
+    """Byte 255 stands for NaN wherever the row is used; the smallest scales, 2^-127 among them, multiply with large ones."""
+    (a, a64), (b, b64) = rows8(300, k, 9, spread=0), rows8(300, k, 10, spread=0)
+    a.scale.view(torch.uint8)[7, -1] = 255
+    b.scale.view(torch.uint8)[299, 0] = 255
+    got = eng.q8_product(a, b).cpu()
+    want = torch.zeros(300, 300, dtype=torch.bool)
+    want[7], want[:, 299] = True, True
+    assert torch.equal(got.isnan(), want)
+    (a, _), (b, _) = rows8(300, k, 11, spread=0), rows8(40, k, 12, spread=0)
+    for byte in (0, 1, 2, 5):
+        low = q8.Q8(a.codes, torch.full_like(a.scale.view(torch.uint8), byte).view(torch.float8_e8m0fnu))
+        high = q8.Q8(b.codes, torch.full_like(b.scale.view(torch.uint8), 240).view(torch.float8_e8m0fnu))
+        close(eng.q8_product(low, high), torch.from_numpy(decode(*low)), torch.from_numpy(decode(*high)), k)
+
+
 def offsets(sizes):
     return torch.tensor([0] + list(np.cumsum(sizes)), dtype=torch.int32).cuda()
 
@@ -273,6 +290,9 @@ def test_clutter_score_nan(eng):
     got = eng.q8_clutter_score(a, b).cpu()
     assert bool(got[1, 3, 4].isnan()) and int(got.isnan().sum()) == 1
     b.codes.view(torch.uint8)[69, 127] = 0x7f
+    assert bool(eng.q8_clutter_score(a, b).isnan().all())
+    (b, _) = rows8(70, 128, 42)
+    b.scale.view(torch.uint8)[0, 0] = 255
     assert bool(eng.q8_clutter_score(a, b).isnan().all())
 
 
@@ -436,6 +456,7 @@ def test_refusals(eng):
         (_lib.NemoHipError, lambda: eng.quantize(torch.zeros(4, 24, device='cuda'))),
         (_lib.NemoHipError, lambda: eng.quantize(torch.zeros(4 * 128 + 1, device='cuda')[1:].view(4, 128))),
         (TypeError, lambda: eng.dequantize(a.codes.view(torch.uint8), a.scale)),
+        (TypeError, lambda: eng.dequantize(*maps, slots=[0])),
         (ValueError, lambda: eng.dequantize(a.codes, a.scale[:-1])),
         (TypeError, lambda: eng.dequantize(a.codes, a.scale, dtype=torch.float64)),
         (ValueError, lambda: eng.dequantize(*a, channel_major=True)),

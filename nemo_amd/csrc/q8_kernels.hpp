@@ -88,7 +88,8 @@ __device__ __forceinline__ bool q8_overwritten(const int32_t *slots, int i, int 
 // ---------------------------------------------------------------- quantise, channels contiguous
 // x [n][rows][C] -> q [slot][rows][C], e [slot][rows][nb].  16 lanes own a block of 128 channels, 8 numbers a lane (fp32: 4
 // in either half of the block, so that every load instruction reads whole cache lines), its maximum goes through four
-// rotations inside the 16 lanes.
+// rotations inside the 16 lanes.  Bound by memory: 33 maps of 160 x 200 x 256 in bf16, 813 MB, 152 us = 5.3 TB/s (a large copy moves
+// 4.7); with the loads of 2 bytes or not in flight together it took 350.
 constexpr int Q8_QU = 4;  // blocks per 16 lanes: their loads are all in flight before the first is used
 template <class TT>
 __global__ __launch_bounds__(256) void q8_quantize_kernel(const typename TT::T *__restrict__ x, int n, int rows, int C, int nb, unsigned chunks,
@@ -159,7 +160,8 @@ __global__ __launch_bounds__(256) void q8_quantize_kernel(const typename TT::T *
 // x [n][C][rows] -> the same q and e (the layout a backbone leaves and a feature record holds).  A workgroup owns 64 PX pixels and one
 // block of 128 channels, a wave 32 of the channels: a lane's numbers are of PX pixels (one 4-byte load a channel: PX = 1 for fp32, 2 for
 // 16 bits, where loads of 2 bytes reached 2.3 TB/s), so the maximum needs one exchange between the waves; the codes go through LDS so that a
-// pixel's 128 bytes leave as one line.
+// pixel's 128 bytes leave as one line.  Bound by memory: 512 fp32 maps of 80 x 100 x 128, 2.63 GB, 497 us = 5.3 TB/s; one map of
+// 32 x 84 x 128 takes 3.4 us, a launch.
 template <class TT>
 __global__ __launch_bounds__(256) void q8_quantize_t_kernel(const typename TT::T *__restrict__ x, int n, int rows, int C, int nb, unsigned tiles,
                                                             const int32_t *__restrict__ slots, int n_slots, uint8_t *__restrict__ q,
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(256) void q8_quantize_t_kernel(const typename TT::T
 
 // ---------------------------------------------------------------- read back, channels contiguous
 // q [slot][rows][C], e -> x [n][rows][C]; a lane reads as many codes as make 16 bytes of numbers, Q8_DU times.  An image without a slot
-// reads zeros.
+// reads zeros.  Bound by memory: 512 maps of 80 x 100 x 128 to fp32, 2.63 GB, 473 us = 5.5 TB/s; one of them 3.8 us.
 constexpr int Q8_DU = 4;
 template <class TT>
 __global__ __launch_bounds__(256) void q8_dequantize_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ e, int rows, int C, int nb,
@@ -290,7 +292,8 @@ __global__ __launch_bounds__(256) void q8_dequantize_kernel(const uint8_t *__res
 // q [slot][rows][C], e -> x [n][C][rows]: 256 pixels x 128 channels through LDS, whose rows of 33 words let the lanes of a wave read one word
 // each of different pixels.  A lane writes PX numbers of a channel, the waves neighbouring pixels: 1 KB (fp32) or 512 bytes of a channel
 // leave at about the same time, and the tiles of a channel follow each other on one XCD (workgroup b runs on XCD b % 8), because lines that
-// are filled in parts cost the memory several times their bytes.
+// are filled in parts cost the memory several times their bytes.  40 maps of 97 x 101 x 208, whose channels begin anywhere in a line: 102 us
+// to fp32 (4.0 TB/s), 74 to bf16.
 template <class TT>
 __global__ __launch_bounds__(256) void q8_dequantize_t_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ e, int rows, int C, int nb,
                                                               unsigned tiles, unsigned n_blocks, const int32_t *__restrict__ slots, int n_slots,
@@ -523,6 +526,8 @@ __device__ __forceinline__ void q8_store(typename TT::T *out, int ld, int m0, in
 // ahead, and turned in LDS of its own (read by rows, a load instruction touches 32 lines for 32 bytes of each: 16 blocks of one tile took
 // 18 us that way).  KS = 1: `across` of the 4 waves of a workgroup stand side by side, the others below them.  KS = 4, for long rows: they deal the blocks of the same tile
 // among them, and their sums are added in the order of the waves.
+// Bound by the launch and the way to memory and back: 1 x 1088 x 128 3.6 us, 1 x 128 x 2048 4.9 (12.4 before the waves shared
+// the blocks), 12 groups of up to 40 rows x up to 1100 4.8.
 template <class TT, int KS>
 __global__ __launch_bounds__(256) void q8_product_few_kernel(Q8Args A, int across, typename TT::T *__restrict__ out) {
   __shared__ __align__(16) uint8_t turn[4][2][4096];
@@ -677,7 +682,12 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
 // operations, but leaves 4 bytes), so the work is cut for the stores: the 8 waves of a workgroup own neighbouring columns of the same
 // rows, 64 each, whose bank rows stay in registers, and the rows pass by, up to 256 of them copied to LDS as codes before the
 // first product.  A workgroup then writes 512 columns of 32 rows at about the same time, which fills whole lines also where out's rows
-// begin in the middle of one, and waits for no store.  With wc < 8, 8 / wc waves share the columns and take the row tiles in turn.
+// begin in the middle of one, and waits for no store.  With wc < 8, 8 / wc waves share the columns and take the row tiles in turn; so do
+// all 8 where a bank's last columns are few (262144 rows x 1088: bf16 136 -> 125 us, f32 227 -> 213; x 640 f32 152 -> 134; x 1095, whose lines
+// are shared between the cuts, bf16 182 -> 186, f32 240 -> 242).  f32 reaches 5.2 TB/s of results where rows are whole lines and 4.7 where
+// they are not (x 1095), bf16 4.5 and 3.1: a line that leaves in two parts costs about as much as two (stores alone, without the products,
+// reach 5.4 and 3.2 on the same rows in bf16).  Twice the columns a wave, so that a bf16 row leaves in the same 256 bytes as an f32 one, takes 216
+// registers and leaves one workgroup a compute unit: 200 us for 262144 x 1095, 250 for the mixed batch that takes 155 this way.
 constexpr int Q8_PR = 256;  // rows per workgroup, at most
 template <class TT, bool TAIL>
 __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int tiles, int cuts, int wc, int rt, typename TT::T *__restrict__ out) {
@@ -691,8 +701,10 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
   Q8Seg S;
   if (!q8_find<8>(A, id / cuts, 32 * rt, S)) return;
   const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cols = min(S.n1 - S.n0, A.n_cols), n0 = ((int)(id % cuts) * wc + w % wc) * 32 * NT, m1 = min(S.r1, S.r0 + 32 * rt);
-  if ((int)(id % cuts) * wc * 32 * NT >= cols) return;
+  const int cols = min(S.n1 - S.n0, A.n_cols), c0 = (int)(id % cuts) * wc * 32 * NT, m1 = min(S.r1, S.r0 + 32 * rt);
+  if (c0 >= cols) return;
+  while (wc > 1 && cols - c0 <= 16 * NT * wc) wc /= 2;  // a bank's last columns
+  const int n0 = c0 + (w % wc) * 32 * NT;
   uint32_t e[Rows::NE];
   L.copy(0, A.a + (size_t)S.r0 * A.K, A.ae + (size_t)S.r0 * NB, A.K, m1 - S.r0, 0, 32 * rt, tid, e);
   // The wave's 32 NT bank rows, 8 KB, read in order of addresses and turned in LDS by halves: lanes i < 16 have their rows in the first
@@ -753,7 +765,10 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
 
 // Long rows (K > 128): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS.  There is
 // one buffer: a wave reads its 16 KB of a step into registers, and once all waves have, the next step is copied under the widening (128
-// instructions a wave) and the products (32, 1024 cycles).
+// instructions a wave) and the products (32, 1024 cycles).  172032 x 128 x 2048 (443 MB, 90 GFLOP): 106-110 us = 4.1 TB/s and 0.83
+// PFLOP/s.  Bound by the waits for a step's codes, 16 KB of a and as much of b for 36 us of matrix instructions in all; 1344
+// workgroups in places for 768 leave the last round three quarters full.  Two buffers and two workgroups a compute unit took 155, a step
+// copied before it is read into registers 135; a fourth workgroup (spills) 147.
 template <class TT>
 __global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
   __shared__ __align__(16) uint8_t codes[2][128 * Q8_BLOCK];  // a, b
@@ -904,6 +919,7 @@ __global__ __launch_bounds__(512, T * NB >= 2 ? 2 : 4) void q8_score_kernel(Q8Ar
   }
 }
 // Few pixels: the 8 waves share 32 pixels and deal the bank's row tiles among them; the bank comes straight from memory, a tile ahead.
+// Bound by the launch: one map of 80 x 100 against one vector 3.2 us.
 template <int NB>
 __global__ __launch_bounds__(512) void q8_score_few_kernel(Q8Args A, float *__restrict__ out) {
   constexpr int RB = Q8_BLOCK * NB;

@@ -30,7 +30,7 @@ __device__ __forceinline__ int q8_exponent(uint32_t amax) {
 __device__ __forceinline__ float q8_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 // the number a scale byte stands for (byte 0: 2^-127, byte 255: NaN; quantising writes neither)
 __device__ __forceinline__ float q8_scale(uint32_t byte) {
-  return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+  return __uint_as_float(byte << 23 | (byte - 1 >= 254 ? 0x00400000u : 0u));
 }
 __device__ __forceinline__ uint32_t q8_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 // four numbers, already times 2^-e, to four codes
@@ -763,16 +763,41 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
   }
 }
 
-// Long rows (K > 128): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS.  There is
-// one buffer: a wave reads its 16 KB of a step into registers, and once all waves have, the next step is copied under the widening (128
-// instructions a wave) and the products (32, 1024 cycles).  172032 x 128 x 2048 (443 MB, 90 GFLOP): 106-110 us = 4.1 TB/s and 0.83
-// PFLOP/s.  Bound by the waits for a step's codes, 16 KB of a and as much of b for 36 us of matrix instructions in all; 1344
-// workgroups in places for 768 leave the last round three quarters full.  Two buffers and two workgroups a compute unit took 155, a step
-// copied before it is read into registers 135; a fourth workgroup (spills) 147.
+// Long rows (K > 128): tiles of 128 x 128, 4 waves of 64 x 64, 128 channels a step, whose codes the memory unit copies to LDS: a's, which
+// come from far, two steps ahead into two buffers, b's, which the other tiles keep near, one step into one, 48 KB for three workgroups a compute
+// unit.  A wave reads its 16 KB of a step into registers, and once all waves have, the next copies start under the widening (128
+// instructions a wave) and the products (32, 1024 cycles).
+// Bound by the matrix units and the widening beside them: 8192 x 8192 x 2048 253-257 us = 1.08 PFLOP/s, 172032 x 128 x 2048 (443 MB, 90
+// GFLOP) 106-120 us = 0.75-0.85 PFLOP/s and 4 TB/s, whose 1344 workgroups in places for 768 leave the second round three quarters full.  Two
+// buffers of both and two workgroups a compute unit took 155 us for the latter, one buffer copied before it is read into registers 135;
+// one buffer copied after it the same as now, but 346 us for 262144 x 1088 x 256 (now 295) and 200 for 50000 x 2600 x 512 (now 189).
+// The wave's codes of a step (x: 32 rows and the 32 behind them, y: the even and the odd of 64 rows) out of LDS.  The compiler would wait for
+// every copy under way before a read of LDS that it sees; the wait for the reads stands in the same block.
+__device__ __forceinline__ void q8_read_step(uint32_t ax, uint32_t ay, Q8Raw (&x)[2], Q8Raw (&y)[2]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %10 offset:4096\n\tds_read_b128 %7, %11 offset:4096\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0].v[0]), "=&v"(x[0].v[1]), "=&v"(x[0].v[2]), "=&v"(x[0].v[3]), "=&v"(x[1].v[0]), "=&v"(x[1].v[1]), "=&v"(x[1].v[2]), "=&v"(x[1].v[3])
+      : "v"(ax), "v"(ax ^ 32), "v"(ax ^ 64), "v"(ax ^ 96)
+      : "memory");
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %12\n\tds_read_b128 %5, %13\n\tds_read_b128 %6, %14\n\tds_read_b128 %7, %15\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(y[0].v[0]), "=&v"(y[0].v[1]), "=&v"(y[0].v[2]), "=&v"(y[0].v[3]), "=&v"(y[1].v[0]), "=&v"(y[1].v[1]), "=&v"(y[1].v[2]), "=&v"(y[1].v[3])
+      : "v"(ay), "v"(ay ^ 32), "v"(ay ^ 64), "v"(ay ^ 96), "v"(ay ^ 128), "v"(ay ^ 160), "v"(ay ^ 192), "v"(ay ^ 224)
+      : "memory");
+}
+__device__ __forceinline__ void q8_barrier() {  // no wait for copies under way
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 template <class TT>
 __global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
-  __shared__ __align__(16) uint8_t codes[2][128 * Q8_BLOCK];  // a, b
-  __shared__ float scale[2][128];
+  constexpr int STEP = 128 * Q8_BLOCK;
+  __shared__ __align__(256) uint8_t codes[3][STEP];  // a, a of the next step, b
   // the column tiles of the same rows follow each other on one XCD, whose L2 keeps the rows of a
   const unsigned n = (unsigned)tiles * (unsigned)cuts, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= n) return;
@@ -783,49 +808,57 @@ __global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int t
   if (n0 >= cols) return;
   // the thread's 16-byte pieces of a step, 32 rows apart: where their rows begin behind the tile's first (128 rows: 32 bits)
   const uint8_t *ta = A.a + (size_t)S.r0 * A.K, *tb = A.b + ((size_t)S.n0 + n0) * A.K;
-  uint32_t pa[4], pb[4];
   int r0, q;
   q8_at<1>(tid, r0, q);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    pa[j] = (uint32_t)min(r0 + 32 * j, m1 - 1 - S.r0) * (uint32_t)A.K;
-    pb[j] = (uint32_t)min(r0 + 32 * j, cols - 1 - n0) * (uint32_t)A.K;
-  }
-  const uint8_t *pe = tid < 128 ? A.ae + (size_t)min(S.r0 + tid, m1 - 1) * A.nb : A.be + ((size_t)S.n0 + min(n0 + tid - 128, cols - 1)) * A.nb;
-  uint32_t e;
-  auto copy = [&](int b) {
-    const uint32_t k = (uint32_t)min(b * Q8_BLOCK + 16 * q, A.K - 16);  // past the end of a row: its last piece, taken for zeros below
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      q8_copy16(ta + (pa[j] + k), &codes[0][4096 * j + 1024 * w]);
-      q8_copy16(tb + (pb[j] + k), &codes[1][4096 * j + 1024 * w]);
-    }
-    e = pe[b];
-  };
+  uint32_t pa = (uint32_t)r0 * (uint32_t)A.K, pb = pa;
+  const uint32_t last_a = (uint32_t)min(m1 - 1 - S.r0, 127) * (uint32_t)A.K, last_b = (uint32_t)min(cols - 1 - n0, 127) * (uint32_t)A.K;
   const int mw = 64 * (w >> 1), nw = 64 * (w & 1);  // the wave's corner of the tile
+  // its scales: rows i and i + 32 of a's, 2 i and 2 i + 1 of b's
+  const uint8_t *tae = A.ae + (size_t)S.r0 * A.nb, *tbe = A.be + ((size_t)S.n0 + n0) * A.nb;
+  uint32_t pea = (uint32_t)(mw + i) * (uint32_t)A.nb, peb = (uint32_t)(nw + 2 * i) * (uint32_t)A.nb;
+  const uint32_t last_ea = (uint32_t)min(m1 - 1 - S.r0, 127) * (uint32_t)A.nb, last_eb = (uint32_t)min(cols - 1 - n0, 127) * (uint32_t)A.nb;
+  uint32_t e[4];
+  auto piece = [&](int b) { return (uint32_t)min(b * Q8_BLOCK + 16 * q, A.K - 16); };  // past the end of a row: its last piece, taken for zeros below
+  auto copy_a = [&](int b) {
+    const uint32_t k = piece(b);
+    __builtin_amdgcn_sched_barrier(0);  // the wait above counts on these being the last
+    asm("" : "+v"(pa));  // the four places are computed anew: kept, they would cost the third workgroup a compute unit
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q8_copy16(ta + (min(pa + 32 * j * (uint32_t)A.K, last_a) + k), &codes[b & 1][4096 * j + 1024 * w]);
+  };
+  auto copy_b = [&](int b) {
+    const uint32_t k = piece(b);
+    asm("" : "+v"(pb), "+v"(pea), "+v"(peb));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q8_copy16(tb + (min(pb + 32 * j * (uint32_t)A.K, last_b) + k), &codes[2][4096 * j + 1024 * w]);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      e[s] = tae[min(pea + 32 * s * (uint32_t)A.nb, last_ea) + (uint32_t)b];
+      e[2 + s] = tbe[min(peb + s * (uint32_t)A.nb, last_eb) + (uint32_t)b];
+    }
+  };
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&codes[0][0];
+  const uint32_t ax = lds + (uint32_t)q8_place<1>(mw + i, h), ay = lds + 2 * STEP + (uint32_t)q8_place<1>(nw + 2 * i, h);
   f16v acc[2][2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int t = 0; t < 2; ++t) acc[s][t] = q8_zero();
-  copy(0);
-  for (int b = 0; b < A.nb; ++b) {
-    scale[tid >> 7][tid & 127] = q8_scale(e);
-    q8_wait_copies();
-    __syncthreads();
-    const int left = A.K - b * Q8_BLOCK;
-    const float sx[2] = {scale[0][mw + i], scale[0][mw + 32 + i]}, sy[2] = {scale[1][nw + 2 * i], scale[1][nw + 2 * i + 1]};
+  auto step = [&](int b, auto more_a, auto more_b) {
+    __builtin_amdgcn_s_waitcnt(decltype(more_b)::value ? 0x0f74 : 0x0f70);  // vmcnt(4): all but the copies of the next step's a; or (0)
+    q8_barrier();
+    asm volatile("" : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]));  // what is made of them is not made before the wait
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = q8_scale(e[j]);
     Q8Raw x[2], y[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        x[s].v[u] = *(const u4va *)&codes[0][q8_place<1>(mw + 32 * s + i, 2 * u + h)];
-        y[s].v[u] = *(const u4va *)&codes[1][q8_place<1>(nw + 2 * i + s, 2 * u + h)];
-      }
-    __syncthreads();  // the buffer has been read
-    if (b + 1 < A.nb) copy(b + 1);
-    if (left < Q8_BLOCK) {
+    q8_read_step(ax + (uint32_t)(b & 1) * STEP, ay, x, y);
+    q8_barrier();  // the buffers have been read
+    if (decltype(more_b)::value) copy_b(b + 1);
+    if (decltype(more_a)::value) copy_a(b + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    const int left = A.K - b * Q8_BLOCK;
+    if (!decltype(more_b)::value && left < Q8_BLOCK) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (16 * (2 * u + h) >= left) x[0].v[u] = x[1].v[u] = y[0].v[u] = y[1].v[u] = u4va{0, 0, 0, 0};
@@ -834,14 +867,21 @@ __global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int t
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const bf8v x0 = q8_numbers(x[0].v[u][2 * g], x[0].v[u][2 * g + 1], sx[0]), y0 = q8_numbers(y[0].v[u][2 * g], y[0].v[u][2 * g + 1], sy[0]);
+        const bf8v x0 = q8_numbers(x[0].v[u][2 * g], x[0].v[u][2 * g + 1], f[0]), y0 = q8_numbers(y[0].v[u][2 * g], y[0].v[u][2 * g + 1], f[2]);
         acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0, y0, acc[0][0], 0, 0, 0);
-        const bf8v x1 = q8_numbers(x[1].v[u][2 * g], x[1].v[u][2 * g + 1], sx[1]), y1 = q8_numbers(y[1].v[u][2 * g], y[1].v[u][2 * g + 1], sy[1]);
+        const bf8v x1 = q8_numbers(x[1].v[u][2 * g], x[1].v[u][2 * g + 1], f[1]), y1 = q8_numbers(y[1].v[u][2 * g], y[1].v[u][2 * g + 1], f[3]);
         acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1, y0, acc[1][0], 0, 0, 0);
         acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x0, y1, acc[0][1], 0, 0, 0);
         acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x1, y1, acc[1][1], 0, 0, 0);
       }
-  }
+  };
+  copy_a(0);
+  copy_b(0);
+  copy_a(1);  // K > 128: there are two steps
+  int b = 0;
+  for (; b + 2 < A.nb; ++b) step(b, std::true_type(), std::true_type());
+  step(b, std::false_type(), std::true_type());
+  step(b + 1, std::false_type(), std::false_type());
 #pragma unroll
   for (int s = 0; s < 2; ++s)
     if (S.r0 + mw + 32 * s < m1 && n0 + nw < cols)

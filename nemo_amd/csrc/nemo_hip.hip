@@ -1272,9 +1272,10 @@ static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, vo
     else hipLaunchKernelGGL((q8_product_few_kernel<TT, 1>), grid, dim3(256), 0, st, A, across, out);
   } else if (A.nb == 1) {
     // Short rows: 8 waves over 512 columns of a bf16 result (wc = 8), over half of them in f32, two to the same columns: 1 KB of a row
-    // either way.  (262144 rows x 1095 x 128, whose rows begin anywhere in a line: f32 315 us with wc = 8, 233 with 4; bf16 192 and 188, but
-    // 135 and 161 where rows are whole lines.)  Fewer where there are fewer columns.  As many rows to a workgroup, up to 128 (f32) or 256,
-    // as still give a workgroup to every compute unit (8000 x 1088 f32: 128 rows 11.7 us, 64 12.6, 32 15.1).
+    // either way.  (262144 rows x 1095 x 128, whose rows begin anywhere in a line: f32 312 us with wc = 8, 242 with 4; bf16 186 and 204; x 1088,
+    // whole lines: f32 227 and 214, bf16 125 and 155.)  Fewer where there are fewer columns.  As many rows to a workgroup, up to 128 (f32) or
+    // 256, as still give a workgroup to every compute unit (8000 x 1088 f32: 128 rows 11.2 us, 64 11.6, 32 13.8; 262144 x 1088 f32: 213,
+    // 317, 378).
     int wc = sizeof(typename TT::T) == 4 ? 4 : 8;
     while (wc > 1 && A.n_cols <= 64 * (wc / 2)) wc /= 2;
     const size_t cuts = ((size_t)A.n_cols + 64 * wc - 1) / ((size_t)64 * wc);

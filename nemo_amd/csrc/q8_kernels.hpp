@@ -767,10 +767,11 @@ __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int 
 // come from far, two steps ahead into two buffers, b's, which the other tiles keep near, one step into one, 48 KB for three workgroups a compute
 // unit.  A wave reads its 16 KB of a step into registers, and once all waves have, the next copies start under the widening (128
 // instructions a wave) and the products (32, 1024 cycles).
-// Bound by the matrix units and the widening beside them: 8192 x 8192 x 2048 253-257 us = 1.08 PFLOP/s, 172032 x 128 x 2048 (443 MB, 90
-// GFLOP) 106-120 us = 0.75-0.85 PFLOP/s and 4 TB/s, whose 1344 workgroups in places for 768 leave the second round three quarters full.  Two
-// buffers of both and two workgroups a compute unit took 155 us for the latter, one buffer copied before it is read into registers 135;
-// one buffer copied after it the same as now, but 346 us for 262144 x 1088 x 256 (now 295) and 200 for 50000 x 2600 x 512 (now 189).
+// Bound by the copies, above all: 172032 x 128 x 2048 (443 MB, 90 GFLOP) takes 110-120 us = 4 TB/s and 0.8 PFLOP/s, 105 without its products, 80
+// without its stores too (a's codes alone 58, 6 TB/s), but 118 without the reads from LDS and 117 without the widening; 8192 x 8192 x
+// 2048 takes 246-256 us = 1.1 PFLOP/s, 194 and 159 in the same way.  For the former two buffers of both and two workgroups a compute unit took
+// 155, one buffer copied before it is read into registers 135; one buffer copied after it the same as now, but 346 us for 262144 x 1088 x
+// 256 (now 295) and 200 for 50000 x 2600 x 512 (now 186).
 // The wave's codes of a step (x: 32 rows and the 32 behind them, y: the even and the odd of 64 rows) out of LDS.  The compiler would wait for
 // every copy under way before a read of LDS that it sees; the wait for the reads stands in the same block.
 __device__ __forceinline__ void q8_read_step(uint32_t ax, uint32_t ay, Q8Raw (&x)[2], Q8Raw (&y)[2]) {
@@ -798,13 +799,18 @@ template <class TT>
 __global__ __launch_bounds__(256, 2) void q8_product_long_kernel(Q8Args A, int tiles, int cuts, typename TT::T *__restrict__ out) {
   constexpr int STEP = 128 * Q8_BLOCK;
   __shared__ __align__(256) uint8_t codes[3][STEP];  // a, a of the next step, b
-  // the column tiles of the same rows follow each other on one XCD, whose L2 keeps the rows of a
+  // Workgroups that follow each other on an XCD take 4 row tiles with one column tile, then with the next: what its L2 brings of b serves all 4
+  // (30000 x 10300 x 512: 459 us a row tile at a time, 402 by 4, 406 by 8, 431 by 16; 60000 x 1100 x 256, whose column tiles share lines of
+  // the result: 75.4, 75.1 and 78.7).
+  constexpr unsigned GROUP = 4;
   const unsigned n = (unsigned)tiles * (unsigned)cuts, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= n) return;
+  const unsigned first = id / (GROUP * (unsigned)cuts) * GROUP, in = id - first * (unsigned)cuts, high = min(GROUP, (unsigned)tiles - first);
+  const unsigned tile = first + in % high, cut = in / high;
   Q8Seg S;
-  if (!q8_find<4>(A, id / cuts, 128, S)) return;
+  if (!q8_find<4>(A, tile, 128, S)) return;
   const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cols = min(S.n1 - S.n0, A.n_cols), n0 = (int)(id % cuts) * 128, m1 = S.r1;
+  const int cols = min(S.n1 - S.n0, A.n_cols), n0 = (int)cut * 128, m1 = S.r1;
   if (n0 >= cols) return;
   // the thread's 16-byte pieces of a step, 32 rows apart: where their rows begin behind the tile's first (128 rows: 32 bits)
   const uint8_t *ta = A.a + (size_t)S.r0 * A.K, *tb = A.b + ((size_t)S.n0 + n0) * A.K;

@@ -668,12 +668,25 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
       __builtin_memcpy((char GAS *)row + place, &o, sizeof(o));
     }
   } else {
+    // The lanes whose columns all exist still store them together (262144 x 40: bf16 20.8 -> 16.0 us, f32 23 -> 20.0).
+    const int left = n1 - n0 - NT * i, rows = m1 - m0 - 4 * h;
+    auto to = [&](int r) { return (char GAS *)(uintptr_t)(base + (size_t)(8 * (r >> 2) + (r & 3)) * ld) + at; };
+    if (left >= NT) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (n0 + NT * i + t >= n1) break;
+      for (int r = 0; r < 16; ++r) {
+        Q8Out<TT, NT> o;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (m0 + 8 * (r >> 2) + (r & 3) + 4 * h < m1) ((T *)((char *)(base + (size_t)(8 * (r >> 2) + (r & 3)) * ld) + at))[t] = TT::put(acc[t][r]);
+        for (int t = 0; t < NT; ++t) o.v[t] = TT::put(acc[t][r]);
+        if (8 * (r >> 2) + (r & 3) < rows) __builtin_memcpy(to(r), &o, sizeof(o));
+      }
+    } else {  // one lane of either half, at most
+#pragma unroll
+      for (int t = 0; t < NT - 1; ++t) {
+        if (t >= left) break;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + (r & 3) < rows) ((T GAS *)to(r))[t] = TT::put(acc[t][r]);
+      }
     }
   }
 }

@@ -699,8 +699,9 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
 // all 8 where a bank's last columns are few (262144 rows x 1088: bf16 136 -> 125 us, f32 227 -> 213; x 640 f32 152 -> 134; x 1095, whose lines
 // are shared between the cuts, bf16 182 -> 186, f32 240 -> 242).  f32 reaches 5.2 TB/s of results where rows are whole lines and 4.7 where
 // they are not (x 1095), bf16 4.5 and 3.1: a line that leaves in two parts costs about as much as two (stores alone, without the products,
-// reach 5.4 and 3.2 on the same rows in bf16).  Twice the columns a wave, so that a bf16 row leaves in the same 256 bytes as an f32 one, takes 216
-// registers and leaves one workgroup a compute unit: 200 us for 262144 x 1095, 250 for the mixed batch that takes 155 this way.
+// reach 5.4 and 3.2 on the same rows in bf16; a mixed batch of 12 banks into bf16 rows of 1095 takes 158 us, 155 without its products).
+// Twice the columns a wave, so that a bf16 row leaves in the same 256 bytes as an f32 one, takes 216 registers and leaves one workgroup a compute
+// unit: 200 us for 262144 x 1095, 250 for the mixed batch.
 constexpr int Q8_PR = 256;  // rows per workgroup, at most
 template <class TT, bool TAIL>
 __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int tiles, int cuts, int wc, int rt, typename TT::T *__restrict__ out) {

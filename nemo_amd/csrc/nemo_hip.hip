@@ -34,6 +34,7 @@
 
 #include "nemo_hip.h"
 #include "fastdiv.h"
+#include "q8_plan.h"
 
 #include "device_common.hpp"
 #include "eval_pose.hpp"
@@ -1169,7 +1170,6 @@ struct DeviceGuard {
   ~DeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
 };
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
-constexpr size_t Q8_MAX_BLOCKS = (1u << 24) - 1;  // 256 threads each: a launch holds fewer than 2^32 threads
 
 static int q8_check_rows(nemo_ctx *ctx, const char *who, int32_t dtype, int32_t n, int32_t rows, int32_t C, int32_t n_slots, const void *d_x,
                          const void *d_q, const void *d_e) {
@@ -1248,48 +1248,24 @@ static int q8_operands(nemo_ctx *ctx, const char *who, const uint8_t *d_a, const
 
 }  // extern "C"
 
-// Tiles of tm rows that cover M rows cut into segments, wherever the cuts are (one segment: no more than its own).
-static size_t q8_tiles(const Q8Args &A, size_t tm) {
-  return ((size_t)A.M + tm - 1) / tm + (A.row_off ? (size_t)A.n_seg : 0);
-}
 template <class TT>
 static int q8_launch_product(nemo_ctx *ctx, const char *who, const Q8Args &A, void *d_out, void *stream) {
+  const Q8Plan p = q8_plan({A.M, A.n_seg, A.row_off != nullptr, A.n_cols, A.K, (int)sizeof(typename TT::T), ctx->n_cu});
+  if (p.refusal == Q8_WIDE) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %d columns (at most %d)", who, A.n_cols, Q8_MAX_COLS);
+  if (p.refusal == Q8_MANY) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
   const hipStream_t st = (hipStream_t)stream;
   typename TT::T *out = (typename TT::T *)d_out;
-  const size_t chunks = ((size_t)A.n_cols + 127) / 128, cus = (size_t)ctx->n_cu;
-  // Up to 32 columns, or so few rows that 32 x 128 products a workgroup make at most 3 workgroups for 2 compute units, or fewer than 64 rows a
-  // segment: one wave for 32 x 32 (f32 results: 1000 x 1000 x 128 4.3 us that way, 5.9 and 5.7 with the kernels below; 300 x 8000 x 128
-  // 7.1, 6.5 and 6.1; 262144 x 16 x 128 11.5, 21.5 and 20.7).
-  if (A.n_cols <= 32 || 2 * q8_tiles(A, 32) * chunks <= 3 * cus || (size_t)A.M < 64 * (size_t)A.n_seg) {
-    const bool split = A.nb > 2;
-    const int across = A.n_cols <= 32 ? 1 : 4;
-    const size_t few = q8_tiles(A, split ? 32 : 128 / across), cols = split ? ((size_t)A.n_cols + 31) / 32 : across == 1 ? 1 : chunks;
-    if (few > Q8_MAX_BLOCKS || cols > 65535) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
-    const dim3 grid((unsigned)few, (unsigned)cols);
-    if (split) hipLaunchKernelGGL((q8_product_few_kernel<TT, 4>), grid, dim3(256), 0, st, A, across, out);
-    else hipLaunchKernelGGL((q8_product_few_kernel<TT, 1>), grid, dim3(256), 0, st, A, across, out);
-  } else if (A.nb == 1) {
-    // Short rows: 8 waves over 512 columns of a bf16 result (wc = 8), over half of them in f32, two to the same columns: 1 KB of a row
-    // either way.  (262144 rows x 1095 x 128, whose rows begin anywhere in a line: f32 312 us with wc = 8, 242 with 4; bf16 186 and 204; x 1088,
-    // whole lines: f32 227 and 214, bf16 125 and 155.)  Fewer where there are fewer columns.  As many rows to a workgroup, up to 128 (f32) or
-    // 256, as still give a workgroup to every compute unit (8000 x 1088 f32: 128 rows 11.2 us, 64 11.6, 32 13.8; 262144 x 1088 f32: 213,
-    // 317, 378).
-    int wc = sizeof(typename TT::T) == 4 ? 4 : 8;
-    while (wc > 1 && A.n_cols <= 64 * (wc / 2)) wc /= 2;
-    const size_t cuts = ((size_t)A.n_cols + 64 * wc - 1) / ((size_t)64 * wc);
-    int rt = (sizeof(typename TT::T) == 4 ? Q8_PR / 2 : Q8_PR) / 32;
-    while (rt > 8 / wc && rt > 1 && q8_tiles(A, 32 * rt) * cuts < cus) rt /= 2;
-    const size_t tiles = q8_tiles(A, 32 * rt), blocks = (tiles * cuts + 7) / 8 * 8;
-    if (blocks > (1u << 23) - 1) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
-    const dim3 grid((unsigned)blocks), wg(512);
-    if (A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, false>), grid, wg, 0, st, A, (int)tiles, (int)cuts, wc, rt, out);
-    else hipLaunchKernelGGL((q8_product_short_kernel<TT, true>), grid, wg, 0, st, A, (int)tiles, (int)cuts, wc, rt, out);
+  const dim3 grid(p.grid_x, p.grid_y);
+  if (p.kernel == Q8_FEW) {
+    if (p.split) hipLaunchKernelGGL((q8_product_few_kernel<TT, 4>), grid, dim3(256), 0, st, A, p.across, out);
+    else hipLaunchKernelGGL((q8_product_few_kernel<TT, 1>), grid, dim3(256), 0, st, A, p.across, out);
+  } else if (p.kernel == Q8_SHORT) {
+    if (A.K == 128) hipLaunchKernelGGL((q8_product_short_kernel<TT, false>), grid, dim3(512), 0, st, A, (int)p.tiles, (int)p.cuts, p.wc, p.rt, out);
+    else hipLaunchKernelGGL((q8_product_short_kernel<TT, true>), grid, dim3(512), 0, st, A, (int)p.tiles, (int)p.cuts, p.wc, p.rt, out);
   } else {
-    const size_t n = q8_tiles(A, 128), blocks = (n * chunks + 7) / 8 * 8;
-    if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: too many rows or columns for one launch", who);
-    hipLaunchKernelGGL((q8_product_long_kernel<TT>), dim3((unsigned)blocks), dim3(256), 0, st, A, (int)n, (int)chunks, out);
+    hipLaunchKernelGGL((q8_product_long_kernel<TT>), grid, dim3(256), 0, st, A, (int)p.tiles, (int)p.cuts, out);
   }
   HIP_TRY(ctx, hipGetLastError());
   return NEMO_OK;

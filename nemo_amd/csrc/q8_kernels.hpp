@@ -504,7 +504,7 @@ __device__ __forceinline__ f16v q8_zero() {
 }
 
 // Stores one 32 x 32 tile of products: lane l has column l % 32 of rows 8 (r / 4) + 4 (l / 32) + r % 4.  m0, m1, n0 and n1 are the same
-// for the whole wave: a row's address is a scalar, a lane's place in it 32 bits.
+// for the whole wave: a row's address is a scalar, a lane's place in it 32 bits (Q8_MAX_COLS).
 template <class TT>
 __device__ __forceinline__ void q8_store(typename TT::T *out, int ld, int m0, int m1, int n0, int n1, int i, int h, const f16v &acc) {
   typedef typename TT::T T;
@@ -654,7 +654,7 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
   const uint32_t at = (uint32_t)(4 * h * ld + NT * i) * (uint32_t)sizeof(T);
   T *base = out + (size_t)m0 * ld + n0;
   if (m0 + 32 <= m1 && n0 + 32 * NT <= n1) {
-    // A row's address stays a scalar and the lane's place 32 bits, so that the store instruction adds them (the empty asm keeps the compiler
+    // A row's address stays a scalar and the lane's place 32 bits (Q8_MAX_COLS), so that the store instruction adds them (the empty asm keeps the compiler
     // from summing them in vector registers, an instruction and two registers a store).
     uint32_t place = at;
     asm("" : "+v"(place));
@@ -702,7 +702,6 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
 // reach 5.4 and 3.2 on the same rows in bf16; a mixed batch of 12 banks into bf16 rows of 1095 takes 158 us, 155 without its products).
 // Twice the columns a wave, so that a bf16 row leaves in the same 256 bytes as an f32 one, takes 216 registers and leaves one workgroup a compute
 // unit: 200 us for 262144 x 1095, 250 for the mixed batch.
-constexpr int Q8_PR = 256;  // rows per workgroup, at most
 template <class TT, bool TAIL>
 __global__ __launch_bounds__(512, 4) void q8_product_short_kernel(Q8Args A, int tiles, int cuts, int wc, int rt, typename TT::T *__restrict__ out) {
   constexpr int NB = 1, NT = 2;

@@ -1,0 +1,52 @@
+"""8-bit rows at the ends of the ranges that the calls accept."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip('torch')
+
+from nemo_amd import _lib, q8  # noqa: E402
+from tests.test_q8_gpu import close, eng, rows8  # noqa: E402,F401
+
+
+@pytest.fixture(autouse=True)
+def give_back():
+    """Tests here hold up to a third of the memory."""
+    yield
+    torch.cuda.empty_cache()
+
+
+def repeated(q, n):
+    """n rows: those of q over and over."""
+    out = q8.empty((n, q.codes.shape[1]), 'cuda')
+    for to, part in zip(out, q):
+        to, part = to.view(torch.uint8), part.view(torch.uint8)
+        whole = n // len(part) * len(part)
+        to[:whole].view(-1, *part.shape).copy_(part.expand(whole // len(part), *part.shape))
+        to[whole:] = part[:n - whole]
+    return out
+
+
+def check_repeated(got, a64, b64, k):
+    """Column j of the result is that of row j % len(b64): the first ones against 64 bits, the others equal to them."""
+    p = len(b64)
+    first = got[:, :p].contiguous()
+    close(first, a64, b64, k)
+    for m in range(got.shape[0]):
+        whole = got.shape[1] // p * p
+        assert bool((got[m, :whole].view(-1, p) == first[m]).all()), m
+        assert torch.equal(got[m, whole:], first[m, :got.shape[1] - whole]), m
+
+
+def test_widest_rows_of_a_result(eng):  # noqa: F811
+    """64 rows of 2^27 numbers (34 GB): the rows of either half of a tile land where they belong; one column more is refused."""
+    n = 1 << 27
+    (a, a64), (b, b64) = rows8(64, 16, 1), rows8(4099, 16, 2)
+    wide = repeated(b, n + 1)
+    got = eng.q8_product(a, q8.Q8(wide.codes[:n], wide.scale[:n]))
+    check_repeated(got, a64, b64, 16)
+    del got
+    out = torch.full((1, n + 1), 5.0, device='cuda')
+    with pytest.raises(_lib.NemoHipError, match='at most 134217728'):
+        eng.q8_product(q8.Q8(a.codes[:1], a.scale[:1]), wide, out=out)
+    assert bool((out == 5.0).all())

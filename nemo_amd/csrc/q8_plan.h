@@ -45,17 +45,18 @@ inline Q8Plan q8_plan(const Q8Problem &p) {
   const int nb = (p.K + 127) / 128;
   // Up to 32 columns, or so few rows that 32 x 128 products a workgroup make at most 3 workgroups for 2 compute units, or fewer than 64 rows a
   // segment: one wave for 32 x 32 (f32 results: 1000 x 1000 x 128 4.3 us that way, 5.9 and 5.7 with the kernels below; 300 x 8000 x 128
-  // 7.1, 6.5 and 6.1; 262144 x 16 x 128 11.5, 21.5 and 20.7).
+  // 7.1, 6.5 and 6.1; 262144 x 16 x 128 11.5, 21.5 and 20.7).  The others take what does not fit its grid.
   if (p.n_cols <= 32 || 2 * q8_tiles(p, 32) * chunks <= 3 * cus || (size_t)p.M < 64 * (size_t)p.n_seg) {
     r.kernel = Q8_FEW;
     r.split = nb > 2;
     r.across = p.n_cols <= 32 ? 1 : 4;
     r.tiles = q8_tiles(p, r.split ? 32 : 128 / r.across);
     r.cuts = r.split ? ((size_t)p.n_cols + 31) / 32 : r.across == 1 ? 1 : chunks;
-    if (r.tiles > Q8_MAX_BLOCKS || r.cuts > 65535) r.refusal = Q8_MANY;
-    r.grid_x = (unsigned)r.tiles;
-    r.grid_y = (unsigned)r.cuts;
-    return r;
+    if (r.tiles <= Q8_MAX_BLOCKS && r.cuts <= 65535) {
+      r.grid_x = (unsigned)r.tiles;
+      r.grid_y = (unsigned)r.cuts;
+      return r;
+    }
   }
   size_t blocks;
   if (nb == 1) {

@@ -50,3 +50,10 @@ def test_widest_rows_of_a_result(eng):  # noqa: F811
     with pytest.raises(_lib.NemoHipError, match='at most 134217728'):
         eng.q8_product(q8.Q8(a.codes[:1], a.scale[:1]), wide, out=out)
     assert bool((out == 5.0).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('m,n,k', [(1, 65535 * 128 + 1, 16), (2, 65535 * 128 + 259, 128), (63, 65535 * 128 + 130, 32), (1, 65535 * 32 + 1, 272), (5, 65535 * 32 + 4000, 400)])
+def test_few_rows_of_any_width(eng, m, n, k, dtype):  # noqa: F811
+    (a, a64), (b, b64) = rows8(m, k, m + k), rows8(4099, k, k)
+    check_repeated(eng.q8_product(a, repeated(b, n), dtype=dtype), a64, b64, k)

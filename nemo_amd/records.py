@@ -344,10 +344,16 @@ def write_feature_record(path: str, memory: Dict[str, np.ndarray], clutter: Dict
     np.savez(path, **get)
 
 
+def record_file(path: str) -> str:
+    """The file that a record written to `path` becomes: np.savez's rule, .npz is added where it is missing."""
+    path = os.fspath(path)
+    return path if path.endswith('.npz') else path + '.npz'
+
+
 def write_feature_record8(path: str, memory: Dict[str, np.ndarray], clutter: Dict[str, np.ndarray],
                           names: Dict[str, Sequence[str]], features: Dict[str, q8.Q8]) -> None:
     """write_feature_record with maps held in 8 bits: `features[name]` is a pixel-major q8.Q8 [h, w, D] (PoseEngine.quantize or
-    q8.quantize_host), all of one shape.  Banks stay f32."""
+    q8.quantize_host), all of one shape.  Banks stay f32.  The file (record_file(path)) appears whole or not at all."""
     get = {}
     for st in memory:
         get['memory_%s' % st] = np.asarray(memory[st], dtype=np.float32)
@@ -363,14 +369,24 @@ def write_feature_record8(path: str, memory: Dict[str, np.ndarray], clutter: Dic
     if shape is None:
         raise ValueError('no feature maps')
     get['features_8bit'] = np.asarray(shape, dtype=np.int64)
-    os.makedirs(os.path.dirname(os.path.abspath(path)), exist_ok=True)
-    np.savez(path, **get)
+    file = os.path.realpath(record_file(path))
+    os.makedirs(os.path.dirname(file), exist_ok=True)
+    part = '%s.%d.part' % (file, os.getpid())
+    try:
+        with open(part, 'wb') as fh:
+            np.savez(fh, **get)
+        os.replace(part, file)
+    except BaseException:
+        if os.path.exists(part):
+            os.remove(part)
+        raise
 
 
 def quantize_record(src: str, dst: str) -> int:
     """Rewrites a feature record with its maps held in 8 bits (on the host; one image at a time, so that it needs room for the
-    8-bit maps only).  Returns the number of maps."""
-    if os.path.abspath(src) == os.path.abspath(dst):
+    8-bit maps only), as record_file(dst).  Returns the number of maps."""
+    file = record_file(dst)
+    if os.path.realpath(src) == os.path.realpath(file) or (os.path.exists(file) and os.path.samefile(src, file)):
         raise ValueError('quantize_record: %s would overwrite its source' % dst)
     with FeatureRecord(src) as rec:
         if rec.shape8 is not None:

@@ -283,7 +283,7 @@ def main(argv=None):
         if int(os.environ.get('RANK', '0')) != 0:   # one writer
             return 0
         n = records.quantize_record(record_path(args), args.quantize_record)
-        print('%d maps in 8 bits: %s' % (n, args.quantize_record))
+        print('%d maps in 8 bits: %s' % (n, records.record_file(args.quantize_record)))
         return 0
     world = int(os.environ.get('WORLD_SIZE', '1'))
     rank = int(os.environ.get('RANK', '0'))

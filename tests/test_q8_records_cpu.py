@@ -1,0 +1,61 @@
+"""Feature records held in 8 bits: the file that is written, and the one that is read."""
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from nemo_amd import q8, records, solve_all
+from tests.test_q8_cpu import _record
+
+
+@pytest.mark.parametrize('kind', ['same', 'no suffix', 'symlink', 'symlink without suffix', 'link to the folder', 'hard link', 'relative'])
+def test_quantize_record_keeps_its_source(tmp_path, monkeypatch, kind):
+    src, feats, _ = _record(tmp_path, n=3)
+    assert src.endswith('f32.npz')
+    dst = {'same': src, 'no suffix': src[:-4], 'relative': 'f32', 'link to the folder': str(tmp_path / 'sub' / 'f32.npz')}.get(kind, str(tmp_path / 'link.npz'))
+    if kind.startswith('symlink'):
+        os.symlink(src, dst)
+    if kind == 'symlink without suffix':
+        dst = dst[:-4]
+    if kind == 'link to the folder':
+        os.symlink(str(tmp_path), str(tmp_path / 'sub'))
+    if kind == 'hard link':
+        os.link(src, dst)
+    monkeypatch.chdir(tmp_path)
+    before, listed = open(src, 'rb').read(), sorted(os.listdir(tmp_path))
+    with pytest.raises(ValueError, match='overwrite its source'):
+        records.quantize_record(src, dst)
+    with pytest.raises(ValueError, match='overwrite its source'):
+        solve_all.main(['--type_', 'car', '--record_file', src, '--quantize_record', dst])
+    assert open(src, 'rb').read() == before and sorted(os.listdir(tmp_path)) == listed
+
+
+def test_record_file_is_named_and_read(tmp_path, capsys):
+    src, feats, _ = _record(tmp_path, n=3)
+    assert solve_all.main(['--type_', 'car', '--record_file', src, '--quantize_record', str(tmp_path / 'q8')]) == 0
+    file = str(tmp_path / 'q8.npz')
+    assert file in capsys.readouterr().out
+    with records.FeatureRecord(file) as r:
+        assert r.shape8 == (5, 9, 128) and sorted(r.image_keys) == sorted(feats)
+
+
+def test_record_is_written_whole_or_not_at_all(tmp_path, monkeypatch):
+    src, _, _ = _record(tmp_path, n=3)
+    dst = tmp_path / 'q8.npz'
+    records.quantize_record(src, str(dst))
+    before = dst.read_bytes()
+
+    def fails(fh, **arrays):
+        fh.write(b'half')
+        raise OSError('no space')
+    with monkeypatch.context() as m:
+        m.setattr(np, 'savez', fails)
+        with pytest.raises(OSError, match='no space'):
+            records.quantize_record(src, str(dst))
+    assert dst.read_bytes() == before and sorted(os.listdir(tmp_path)) == ['f32.npz', 'q8.npz']
+    os.symlink(str(dst), str(tmp_path / 'name.npz'))          # a link to another file: that file is written
+    records.write_feature_record8(tmp_path / 'name', {}, {}, {}, {'a': q8.quantize_host(torch.ones(2, 3, 128))})
+    with records.FeatureRecord(str(dst)) as r:
+        assert r.shape8 == (2, 3, 128)
+    assert os.path.islink(tmp_path / 'name.npz')

@@ -218,15 +218,17 @@ class BatchPoseSolver:
 
     def solve_all(self, feats: Union[torch.Tensor, q8.Q8], clutter: Optional[torch.Tensor], mesh_idx: Optional[torch.Tensor] = None,
                   img_idx: Optional[torch.Tensor] = None, want_trace=False,
-                  clutter_scores: Optional[torch.Tensor] = None) -> SolveResult:
+                  clutter_scores: Optional[torch.Tensor] = None, clutter8: bool = True) -> SolveResult:
         """feats [n_img,h,w,D] pixel-major f32 on the device; clutter [K,D] (K=1: the reference's
         mean vector; K>1: max over the K vectors, lib/MeshUtils.py:273-275) or, instead, ready-made
         clutter_scores [n_img,h,w] (clutter_scores_by_group); jobs default to image i with mesh mesh_idx[i].
-        feats may be held in 8 bits (engine.quantize, FeatureRecord.upload8): the clutter score reads them as they
-        are, the grid search and the solve the numbers they stand for, f32 for the length of this call."""
+        feats may be held in 8 bits (engine.quantize, FeatureRecord.upload8): the grid search and the solve read the
+        numbers they stand for, f32 for the length of this call.  Their clutter score is made, with clutter8, from the maps
+        as they are and from `clutter` ROUNDED TO 8 BITS as well (q8.py: a number moves by up to 2^-4 of itself), with
+        clutter8=False from the f32 copy and from `clutter` as given."""
         eng = self.engine
         if isinstance(feats, q8.Q8):
-            if not self.cfg.turn_off_clutter and clutter_scores is None:
+            if clutter8 and not self.cfg.turn_off_clutter and clutter_scores is None:
                 clutter_scores = eng.q8_clutter_score(feats, eng.quantize(clutter.reshape(-1, eng.D).contiguous()))
             feats = eng.dequantize(*feats)
         if self.cfg.turn_off_clutter:

@@ -58,6 +58,9 @@ def build_parser():
     p.add_argument('--quantize_record', default='', type=str,
                    help='write the category\'s feature record to this file with its maps held in 8 bits (a quarter of the bytes to read and '
                         'upload; a run on that file solves on the numbers they stand for) and stop')
+    p.add_argument('--clutter8', action='store_true',
+                   help='on a record held in 8 bits, round the clutter vectors to 8 bits too and score the maps as they are (else: the f32 '
+                        'vectors against the numbers that the maps stand for)')
     p.add_argument('--batch', default=256, type=int, help='images per solve launch; the next batch is read and uploaded meanwhile')
     p.add_argument('--streams', default=2, type=int,
                    help='solver contexts, each on a stream of its own, taking the batches in turn: the next batch starts on the '
@@ -130,7 +133,7 @@ def batch_plan(n, batch):
     return plan
 
 
-def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
+def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None, clutter8=True):
     """Clutter score (per subtype) -> grid init -> fused solve for the listed images: [len(names), 10] records.
 
     The images go through in batches (batch_plan): while earlier batches are solved, a helper thread reads the next one
@@ -139,8 +142,13 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
     in 8 bits).  Batches alternate between --streams solver
     contexts, each with its own stream and workspaces: a solve is one workgroup per job for all its steps, so a launch
     ends with its slowest job while most compute units idle; the next batch's launches, queued on the other stream,
-    take those units as they come free.  Batches do not change results (every job is independent)."""
+    take those units as they come free.  Batches do not change results (every job is independent).
+
+    clutter8, of a record held in 8 bits: the clutter score is made from the maps as they are and from the clutter vectors
+    rounded to 8 bits as well (BatchPoseSolver.clutter_banks8), in one launch a batch; else from the f32 copy of the maps that the solve
+    reads and from the vectors as the record holds them."""
     from concurrent.futures import ThreadPoolExecutor
+    banks8 = clutter8 and rec.shape8 is not None
     dev = torch.device(device)
     if dev.index is None:
         dev = torch.device('cuda', torch.cuda.current_device())
@@ -183,7 +191,7 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
             solver, clutter = build_solver(args, rec, subtypes, dev)
             solver.engine.reserve(biggest, int(solver.grid_theta.shape[1]))
             solver.prerender()
-            if rec.shape8 is not None and not solver.cfg.turn_off_clutter:
+            if banks8 and not solver.cfg.turn_off_clutter:
                 clutter = solver.clutter_banks8(clutter)
             ctxs.append((solver, clutter, torch.cuda.Stream(dev) if n_ctx > 1 else main))
         for st in ctxs:
@@ -199,6 +207,8 @@ def solve_shard(args, rec, subtypes, names, mesh_of, device, stats=None):
                 if timed:
                     b0 = torch.cuda.Event(enable_timing=True)
                     b0.record(stream)
+                if isinstance(feats, tuple) and not banks8:
+                    feats = solver.engine.dequantize(*feats)
                 clu = None if solver.cfg.turn_off_clutter else solver.clutter_scores_by_group(feats, mesh_of[lo:hi], clutter)
                 mesh_idx = torch.tensor(mesh_of[lo:hi], dtype=torch.int32, device=dev)
                 res = solver.solve_all(feats, None, mesh_idx, clutter_scores=clu)
@@ -257,8 +267,8 @@ def solve_category(args, device='cuda:0', skip=()):
             names, mesh_of = [names[i] for i in keep], [mesh_of[i] for i in keep]
         if not names:
             return names, mesh_of, np.zeros((0, RECORD_WIDTH), np.float32)
-        recs = run_sharded(len(names), lambda lo, hi: solve_shard(args, rec, subtypes, names[lo:hi], mesh_of[lo:hi], device)[0],
-                           device)
+        recs = run_sharded(len(names), lambda lo, hi: solve_shard(args, rec, subtypes, names[lo:hi], mesh_of[lo:hi], device,
+                                                                  clutter8=getattr(args, 'clutter8', False))[0], device)
     return names, mesh_of, recs.cpu().numpy()
 
 

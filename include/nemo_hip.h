@@ -279,8 +279,8 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
 
 /* d_out[m][n] = <row m of a, row n of b> (the numbers the rows stand for), f32 or bf16 [M][N], accumulated in fp32 on the bf16 matrix
  * cores (the numbers are exact in bf16): features against a vertex or clutter bank, or the 1x1 convolution behind a backbone.
- * Rows of the result have up to 2^27 numbers (here N, below n_cols); NEMO_ERR_UNSUPPORTED beyond, and where a launch does not
- * hold the results (one segment of up to 2^30 - 1024 rows: none that fits 288 GB). */
+ * Here and below, a and b have up to 2^31 - 1024 rows, and rows of the result up to 2^27 numbers (here N, below n_cols);
+ * NEMO_ERR_UNSUPPORTED beyond, and where a launch does not hold the results (one segment of up to 2^30 - 1024 rows: none that fits 288 GB). */
 int nemo_q8_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be,
                     int32_t N, int32_t K, int32_t out_dtype, void *d_out, void *stream);
 /* The same with a bank for each segment of rows: rows d_row_off[s] .. d_row_off[s + 1] of a (i32[n_seg + 1], not decreasing, from

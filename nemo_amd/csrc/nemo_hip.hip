@@ -1190,8 +1190,8 @@ int nemo_quantize(nemo_ctx *ctx, const void *d_x, int32_t dtype, int32_t channel
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
   const size_t px = dtype == NEMO_F32 ? 64 : 128;  // pixels per workgroup of the channel-major kernel
   const size_t per = channel_major ? ((size_t)rows + px - 1) / px : ((size_t)rows * nb + 16 * Q8_QU - 1) / (16 * Q8_QU);
-  const size_t blocks = per * (channel_major ? nb : 1) * n;
-  if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_quantize: too many rows for one launch");
+  const size_t image = per * (channel_major ? nb : 1), blocks = image * n;
+  if (image > Q8_MAX_BLOCKS || blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_quantize: too many rows for one launch");
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
 #define Q8_LAUNCH(TT)                                                                                                             \
@@ -1214,8 +1214,9 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
   if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
   const size_t per = channel_major ? ((size_t)rows + 255) / 256 : ((size_t)rows * (C / (dtype == NEMO_F32 ? 4 : 8)) + 256 * Q8_DU - 1) / (256 * Q8_DU);
-  const size_t blocks = per * (channel_major ? nb : 1) * n;
-  if (blocks > Q8_MAX_BLOCKS) return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_dequantize: too many rows for one launch");
+  const size_t image = per * (channel_major ? nb : 1), blocks = image * n;
+  if (image > Q8_MAX_BLOCKS || blocks > Q8_MAX_BLOCKS - 7)  // channels first: blocks are rounded up to whole eights
+    return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_dequantize: too many rows for one launch");
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
 #define Q8_LAUNCH(TT)                                                                                                             \
@@ -1235,7 +1236,8 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
 static int q8_operands(nemo_ctx *ctx, const char *who, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be,
                        int32_t N, int32_t K, const void *d_out, Q8Args *A) {
   if (M < 0 || N < 0) return fail(ctx, NEMO_ERR_ARG, "%s: negative size", who);
-  if (M > 0x7fffffff) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %lld rows (at most 2^31 - 1)", who, (long long)M);
+  if (!q8_rows_fit(M) || !q8_rows_fit(N))
+    return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %lld rows (at most %d)", who, (long long)(q8_rows_fit(M) ? N : M), Q8_MAX_ROWS);
   if (K < 16 || K > 65536 || K % 16) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %d channels (a multiple of 16, 16 to 65536)", who, K);
   if (M > 0 && (!d_a || !d_ae)) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);
   if (N > 0 && (!d_b || !d_be)) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);

@@ -329,7 +329,7 @@ __global__ __launch_bounds__(256) void q8_dequantize_t_kernel(const uint8_t *__r
   }
   __syncthreads();
   if (p0 + p >= rows) return;
-  const bool whole = p0 + p + PX <= rows;
+  const bool whole = p0 + p <= rows - PX;
   T *xp = x + ((size_t)img * C + b * Q8_BLOCK) * rows + p0 + p;
   constexpr int CH_W = Q8_BLOCK / PX;  // channels of a wave
 #pragma unroll

@@ -8,6 +8,8 @@
 
 constexpr int Q8_PR = 256;                             // rows per workgroup of the short-row kernel, at most
 constexpr size_t Q8_MAX_BLOCKS = (1u << 24) - 1;       // 256 threads each: a launch holds fewer than 2^32 threads
+// Rows of an operand, at most: the kernels count them in an int, up to 1023 past the last one (the last wave's of the score's 1024).
+constexpr int32_t Q8_MAX_ROWS = 0x7fffffff - 1023;
 // Row length of a result, at most: a lane's place behind the first of 32 rows and 64 columns, (4 n_cols + 62) numbers of up to 4 bytes, has
 // to fit 32 bits in the kernels' stores.
 constexpr int32_t Q8_MAX_COLS = 1 << 27;
@@ -32,6 +34,7 @@ struct Q8Plan {
   int wc, rt;          // short: waves over different columns; row tiles of a workgroup
 };
 
+inline bool q8_rows_fit(int64_t n) { return n <= Q8_MAX_ROWS; }
 // Tiles of tm rows that cover the rows, wherever the cuts are (one segment: no more than its own).
 inline size_t q8_tiles(const Q8Problem &p, size_t tm) { return ((size_t)p.M + tm - 1) / tm + (p.ragged ? (size_t)p.n_seg : 0); }
 

@@ -7,3 +7,4 @@ extern "C" void plan(int32_t M, int32_t n_seg, int32_t ragged, int32_t n_cols, i
   for (int64_t x : v) *to++ = x;
 }
 extern "C" int32_t max_cols() { return Q8_MAX_COLS; }
+extern "C" int32_t rows_fit(int64_t n) { return q8_rows_fit(n); }

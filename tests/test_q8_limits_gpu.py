@@ -57,3 +57,34 @@ def test_widest_rows_of_a_result(eng):  # noqa: F811
 def test_few_rows_of_any_width(eng, m, n, k, dtype):  # noqa: F811
     (a, a64), (b, b64) = rows8(m, k, m + k), rows8(4099, k, k)
     check_repeated(eng.q8_product(a, repeated(b, n), dtype=dtype), a64, b64, k)
+
+
+@pytest.mark.parametrize('m,n', [(2 ** 31 - 1023, 8), (2 ** 31 - 1, 8), (8, 2 ** 31 - 1)])
+def test_more_rows_than_are_counted_are_refused(eng, m, n):  # noqa: F811
+    (a, _), (b, _) = rows8(8, 128, 1), rows8(8, 128, 2)
+    out = torch.full((8, 8), 5.0, device='cuda')
+    off = torch.tensor([0, 8], dtype=torch.int32, device='cuda')
+    at = [t.data_ptr() for t in (*a, *b, off, out)]
+    assert eng.lib.nemo_q8_product(eng.ctx, at[0], at[1], m, at[2], at[3], n, 128, 0, at[5], None) < 0
+    assert b'at most 2147482624' in eng.lib.nemo_last_error(eng.ctx)
+    assert eng.lib.nemo_q8_grouped_product(eng.ctx, at[0], at[1], m, at[4], 1, at[2], at[3], n, at[4], 1, None, 128, 0, 8, at[5], None) < 0
+    assert b'at most 2147482624' in eng.lib.nemo_last_error(eng.ctx)
+    images = m // (eng.h * eng.w) + 1
+    assert eng.lib.nemo_q8_clutter_score(eng.ctx, at[0], at[1], images, at[2], at[3], n, None, 1, None, at[5], None) < 0
+    assert b'at most 2147482624' in eng.lib.nemo_last_error(eng.ctx)
+    torch.cuda.synchronize()
+    assert bool((out == 5.0).all())
+
+
+def test_images_of_two_to_the_31_pixels_read_back(eng):  # noqa: F811
+    """One image of 2^31 - 1 pixels, channels first: each channel ends at its own last pixel, and nothing is written behind the image."""
+    rows, c = 2 ** 31 - 1, 16
+    (part, part64) = rows8(4099, c, 3, spread=3)
+    q = repeated(part, rows)
+    flat = torch.full((rows * c + 64,), 123.0, dtype=torch.float16, device='cuda')
+    got = eng.dequantize(q.codes[None], q.scale[None], channel_major=True, out=flat[:rows * c].view(1, c, rows))
+    assert bool((flat[rows * c:] == 123.0).all())
+    want, whole = part64.to(torch.float16).cuda(), rows // 4099 * 4099
+    for k in range(c):
+        assert bool((got[0, k, :whole].view(-1, 4099) == want[:, k]).all()), k
+        assert torch.equal(got[0, k, whole:], want[:rows - whole, k]), k

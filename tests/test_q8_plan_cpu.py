@@ -1,4 +1,5 @@
 """The launch rules of the 8-bit products on the CPU: sizes that no test can hold."""
+import ctypes
 import random
 
 import pytest
@@ -55,3 +56,12 @@ def test_what_fits_the_memory_is_launched(out_bytes):
             assert p.grid_x >= p.tiles * p.cuts and p.grid_x % 8 == 0 and p.grid_y == 1
         assert p.tiles * rows >= M and p.cuts * cols >= n and p.grid_x * threads < 2 ** 32 and p.tiles * p.cuts < 2 ** 31
     assert seen == {FEW, SHORT, LONG}
+
+
+def test_rows_are_counted_in_an_int():
+    """The furthest row that a kernel names is 1023 past the last (score: 8 waves of 4 x 32 pixels from the tile's first on)."""
+    lib = q8_plan.library()
+    top = 2 ** 31 - 1024
+    assert 7 * 4 * 32 + 3 * 32 + 31 == 1023 and top - 1 + 1023 < 2 ** 31
+    for n, fits in ((top, 1), (top + 1, 0), (2 ** 31 - 1, 0), (2 ** 31, 0), (2 ** 32 + 1, 0), (2 ** 40, 0)):
+        assert lib.rows_fit(ctypes.c_int64(n)) == fits

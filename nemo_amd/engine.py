@@ -302,6 +302,12 @@ class PoseEngine:
                 raise ValueError(f'{name}: must rise from 0 or more to at most {end}')
         return at, t.shape[0] - 1
 
+    @staticmethod
+    def _counts(what, *counts):
+        """Sizes that go to the library as int32, which would drop their upper bits without a word."""
+        if max(counts) > 0x7fffffff:
+            raise ValueError(f'{what}: more than 2^31 - 1 of a size: {counts}')
+
     def _done(self, rc, what):
         if rc < 0:
             _lib.check(self.ctx, rc, what)
@@ -330,6 +336,7 @@ class PoseEngine:
         slot_at = self._index(slots, 'slots', n, n_slots)
         if slots is None and not channel_major:   # one run of rows
             n, rows, n_slots = 1, n * rows, 1
+        self._counts('quantize', n, rows, c, n_slots)
         self._done(self.lib.nemo_quantize(self.ctx, at, dtype, channel_major, n, rows, c, slot_at, n_slots, codes, scale, self._raw_stream()),
                    'nemo_quantize')
         return q8.Q8(*out)
@@ -347,6 +354,10 @@ class PoseEngine:
             n = slots.shape[0] if slots.dim() else 0
             slot_at = self._index(slots, 'slots', n, room[0])
         shape = (n, c) + image if channel_major else (n,) + image + (c,)
+        rows, n_images, n_slots = math.prod(image), n, room[0]
+        if slots is None and not channel_major:   # one run of rows
+            n_images, rows, n_slots = 1, n * rows, 1
+        self._counts('dequantize', n_images, rows, c, n_slots)
         if out is None:
             out = self._empty(shape, dtype)
         kind = self._DTYPES.get(out.dtype)
@@ -355,10 +366,7 @@ class PoseEngine:
         at = self._ready(out, out.dtype, 'out')
         if out.shape != shape:
             raise ValueError(f'out: expected {tuple(shape)}, got {tuple(out.shape)}')
-        rows, n_slots = math.prod(image), room[0]
-        if slots is None and not channel_major:
-            n, rows, n_slots = 1, n * rows, 1
-        self._done(self.lib.nemo_dequantize(self.ctx, codes_at, scale_at, slot_at, n_slots, n, rows, c, kind, channel_major, at,
+        self._done(self.lib.nemo_dequantize(self.ctx, codes_at, scale_at, slot_at, n_slots, n_images, rows, c, kind, channel_major, at,
                                             self._raw_stream()), 'nemo_dequantize')
         return out
 
@@ -378,6 +386,7 @@ class PoseEngine:
         bshape, bc, be = self._q8(b, 'b')
         if len(bshape) != 2 or bshape[1] != k:
             raise ValueError(f'b: expected [N, {k}], got {tuple(bshape)}')
+        self._counts('q8_product', bshape[0], k)
         out, at, kind = self._product_out(out, (*m, bshape[0]), dtype, False)
         self._done(self.lib.nemo_q8_product(self.ctx, ac, ae, math.prod(m), bc, be, bshape[0], k, kind, at, self._raw_stream()), 'nemo_q8_product')
         return out
@@ -396,6 +405,7 @@ class PoseEngine:
         of_at = self._index(bank_of, 'bank_of', n_seg, n_banks)
         if n_cols is None:
             n_cols = out.shape[1] if out is not None and out.dim() == 2 else N
+        self._counts('q8_grouped_product', n_seg, N, n_banks, K, int(n_cols))
         out, at, kind = self._product_out(out, (M, int(n_cols)), dtype, True)
         self._done(self.lib.nemo_q8_grouped_product(self.ctx, ac, ae, M, row_at, n_seg, bc, be, N, bank_at, n_banks, of_at, K, kind, out.shape[1], at,
                                                     self._raw_stream()), 'nemo_q8_grouped_product')
@@ -413,6 +423,7 @@ class PoseEngine:
             raise ValueError(f'cbank: expected [K, {self.D}], got {tuple(bshape)}')
         n, (bank_at, n_banks) = fshape[0], (None, 1) if bank_offsets is None else self._offsets(bank_offsets, 'bank_offsets', bshape[0])
         of_at = self._index(bank_of, 'bank_of', n, n_banks)
+        self._counts('q8_clutter_score', n, bshape[0], n_banks)
         out, at, kind = self._product_out(out, (n, self.h, self.w), torch.float32, bank_of is not None)
         if kind:
             raise TypeError('out: expected torch.float32')

@@ -46,12 +46,16 @@ class FeatureRecord:
         self._z = np.load(path, allow_pickle=False)
         keys = list(self._z.files)
         self.subtypes = sorted(k[len('memory_'):] for k in keys if k.startswith('memory_'))
-        meta = {p + s for s in self.subtypes for p in ('memory_', 'clutter_', 'names_')} | {'features_8bit'}
+        meta = {p + s for s in self.subtypes for p in ('memory_', 'clutter_', 'names_')}
+        # (h, w, D) of the maps of a record held in 8 bits, else None (a map [D, h, w] of that name is an image like others)
+        mark = self._z['features_8bit'] if 'features_8bit' in keys else None
+        self.shape8 = None
+        if mark is not None and not (mark.ndim == 3 and mark.dtype.kind == 'f'):
+            if mark.shape != (3,) or mark.dtype.kind not in 'iu' or mark.min() < 1:
+                raise ValueError('%s: features_8bit is not (h, w, D)' % path)
+            self.shape8 = tuple(int(v) for v in mark)
+            meta.add('features_8bit')
         self.image_keys = [k for k in keys if k not in meta]
-        # (h, w, D) of the maps of a record held in 8 bits, else None
-        self.shape8 = tuple(int(v) for v in self._z['features_8bit']) if 'features_8bit' in keys else None
-        if self.shape8 is not None and (len(self.shape8) != 3 or min(self.shape8) < 1):
-            raise ValueError('%s: features_8bit is not (h, w, D)' % path)
 
     def memory(self, subtype: str) -> np.ndarray:
         return np.ascontiguousarray(self._z['memory_%s' % subtype], dtype=np.float32)
@@ -361,6 +365,8 @@ def write_feature_record8(path: str, memory: Dict[str, np.ndarray], clutter: Dic
         get['names_%s' % st] = np.asarray(list(names[st]), dtype=str)
     shape = None
     for n, f in features.items():
+        if n == 'features_8bit':
+            raise ValueError('a map cannot be named %r: that is the mark of a record held in 8 bits' % n)
         if f.codes.dim() != 3 or tuple(f.codes.shape) != (shape or tuple(f.codes.shape)) or \
                 tuple(f.scale.shape) != tuple(f.codes.shape[:2]) + (q8.n_blocks(f.codes.shape[2]),):
             raise ValueError('map %r: expected [h, w, D] of one shape, got %s' % (n, tuple(f.codes.shape)))

@@ -59,3 +59,23 @@ def test_record_is_written_whole_or_not_at_all(tmp_path, monkeypatch):
     with records.FeatureRecord(str(dst)) as r:
         assert r.shape8 == (2, 3, 128)
     assert os.path.islink(tmp_path / 'name.npz')
+
+
+def test_an_image_may_be_named_like_the_mark(tmp_path):
+    """A map called features_8bit in an f32 record is an image; a record in 8 bits cannot hold it."""
+    rng = np.random.default_rng(1)
+    feats = {n: rng.standard_normal((128, 4, 5)).astype(np.float32) for n in ('a', 'features_8bit')}
+    src, dst = str(tmp_path / 'f32.npz'), tmp_path / 'q8.npz'
+    records.write_feature_record(src, {}, {}, {}, feats)
+    with records.FeatureRecord(src) as r:
+        assert r.shape8 is None and sorted(r.image_keys) == sorted(feats) and r.feature_shape('features_8bit') == (128, 4, 5)
+        assert all(np.array_equal(r.feature(n), f) for n, f in feats.items())
+        got = r.upload_pixel_major(['features_8bit', 'a'], 'cpu')
+        assert np.array_equal(got[0].numpy(), feats['features_8bit'].transpose(1, 2, 0))
+    with pytest.raises(ValueError, match='cannot be named'):
+        records.quantize_record(src, str(dst))
+    assert not dst.exists()
+    for mark in (np.array([5, 9]), np.array([5, 0, 128]), np.array([5.0, 9.0, 128.0]), np.int64(3)):
+        np.savez(dst, features_8bit=mark)
+        with pytest.raises(ValueError, match='is not'):
+            records.FeatureRecord(str(dst))

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import os
 import struct
+import threading
 import time
 import zipfile
 from concurrent.futures import ThreadPoolExecutor
@@ -43,6 +44,7 @@ class FeatureRecord:
 
     def __init__(self, path: str):
         self.path = path
+        self._lock = threading.Lock()   # of the directory that _layout keeps: threads may ask for it first at once
         self._z = np.load(path, allow_pickle=False)
         keys = list(self._z.files)
         self.subtypes = sorted(k[len('memory_'):] for k in keys if k.startswith('memory_'))
@@ -91,11 +93,13 @@ class FeatureRecord:
     def _layout(self, name: str):
         """(byte offset of the array data in the .npz, shape) of a STORED little-endian f32 (8-bit record: u8) C-order member, else None
         (compressed record, other dtype: the caller falls back to the zipfile path)."""
-        if not hasattr(self, '_zinfo'):
-            self._layouts, self._headers = {}, {}
-            self._fd = os.open(self.path, os.O_RDONLY)
-            with zipfile.ZipFile(self.path) as zf:
-                self._zinfo = {i.filename: i for i in zf.infolist()}   # last: its presence says that the rest is there
+        with self._lock:
+            if not hasattr(self, '_zinfo'):
+                with zipfile.ZipFile(self.path) as zf:
+                    zinfo = {i.filename: i for i in zf.infolist()}
+                self._layouts, self._headers = {}, {}
+                self._fd = os.open(self.path, os.O_RDONLY)
+                self._zinfo = zinfo
         if name in self._layouts:
             return self._layouts[name]
         info = self._zinfo.get(name + '.npy')
@@ -194,9 +198,10 @@ class FeatureRecord:
         self._forget()
 
     def _forget(self):
-        if hasattr(self, '_zinfo'):
-            del self._zinfo      # asked for a layout again, the record opens its file again
-            os.close(self._fd)
+        with self._lock:
+            if hasattr(self, '_zinfo'):
+                del self._zinfo      # asked for a layout again, the record opens its file again
+                os.close(self._fd)
 
     def __del__(self):
         self._forget()

@@ -1,5 +1,9 @@
 """Feature records held in 8 bits: the file that is written, and the one that is read."""
 import os
+import threading
+import time
+import zipfile
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -79,3 +83,42 @@ def test_an_image_may_be_named_like_the_mark(tmp_path):
         np.savez(dst, features_8bit=mark)
         with pytest.raises(ValueError, match='is not'):
             records.FeatureRecord(str(dst))
+
+
+def open_files():
+    return len(os.listdir('/proc/self/fd'))
+
+
+def test_directory_of_a_record_leaves_no_file_open(tmp_path, monkeypatch):
+    """Asked for at once by several threads, or in vain: one descriptor at most, none after close."""
+    src, feats, _ = _record(tmp_path, n=3)
+    before = open_files()
+    r = records.FeatureRecord(src)
+    kept = open_files()
+    wait, real = threading.Barrier(8), zipfile.ZipFile
+
+    def slow(*a, **k):
+        time.sleep(0.05)
+        return real(*a, **k)
+    monkeypatch.setattr(records.zipfile, 'ZipFile', slow)
+
+    def ask(name):
+        wait.wait()
+        return r._layout(name)
+    with ThreadPoolExecutor(8) as pool:
+        got = list(pool.map(ask, ['img%d' % (i % 3) for i in range(8)]))
+    assert all(g[1] == (128, 5, 9) for g in got) and got[0] == got[3] == got[6] != got[1]
+    assert open_files() == kept + 1
+    r.close()
+    assert open_files() == before
+    r = records.FeatureRecord(src)
+
+    def broken(*a, **k):
+        raise zipfile.BadZipFile('no directory')
+    monkeypatch.setattr(records.zipfile, 'ZipFile', broken)
+    for _ in range(3):
+        with pytest.raises(zipfile.BadZipFile):
+            r._layout('img0')
+    assert open_files() == kept
+    r.close()
+    assert open_files() == before

@@ -1177,7 +1177,7 @@ static int q8_check_rows(nemo_ctx *ctx, const char *who, int32_t dtype, int32_t 
   if (n < 0 || rows < 0 || n_slots < 0) return fail(ctx, NEMO_ERR_ARG, "%s: negative size", who);
   if (C < 16 || C > 65536 || C % 16) return fail(ctx, NEMO_ERR_UNSUPPORTED, "%s: %d channels (a multiple of 16, 16 to 65536)", who, C);
   if (n == 0 || rows == 0) return NEMO_OK;
-  if (!d_x || !d_q || !d_e) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);
+  if (!d_x || (n_slots > 0 && (!d_q || !d_e))) return fail(ctx, NEMO_ERR_ARG, "%s: null buffer", who);  // a cache without slots may be null
   if (!aligned16(d_x) || !aligned16(d_q)) return fail(ctx, NEMO_ERR_ARG, "%s: buffers must be 16-byte aligned", who);
   return NEMO_OK;
 }
@@ -1186,7 +1186,7 @@ int nemo_quantize(nemo_ctx *ctx, const void *d_x, int32_t dtype, int32_t channel
                   int32_t n_slots, uint8_t *d_q, uint8_t *d_e, void *stream) {
   if (!ctx) return fail(nullptr, NEMO_ERR_ARG, "nemo_quantize: null ctx");
   const int rc = q8_check_rows(ctx, "nemo_quantize", dtype, n, rows, C, n_slots, d_x, d_q, d_e);
-  if (rc != NEMO_OK || n == 0 || rows == 0) return rc;
+  if (rc != NEMO_OK || n == 0 || rows == 0 || n_slots == 0) return rc;
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
   const size_t px = dtype == NEMO_F32 ? 64 : 128;  // pixels per workgroup of the channel-major kernel
   const size_t per = channel_major ? ((size_t)rows + px - 1) / px : ((size_t)rows * nb + 16 * Q8_QU - 1) / (16 * Q8_QU);

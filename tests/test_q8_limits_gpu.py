@@ -88,3 +88,13 @@ def test_images_of_two_to_the_31_pixels_read_back(eng):  # noqa: F811
     for k in range(c):
         assert bool((got[0, k, :whole].view(-1, 4099) == want[:, k]).all()), k
         assert torch.equal(got[0, k, whole:], want[:rows - whole, k]), k
+
+
+@pytest.mark.parametrize('channel_major', [False, True])
+def test_cache_without_slots(eng, channel_major):  # noqa: F811
+    """Every slot is outside such a cache: nothing is written, zeros are read."""
+    cache, slots = q8.empty((0, 5, 144), 'cuda'), torch.tensor([0, -1, 3], dtype=torch.int32, device='cuda')
+    x = torch.randn((3, 144, 5) if channel_major else (3, 5, 144), device='cuda')
+    assert eng.quantize(x, channel_major=channel_major, slots=slots, out=cache).codes.shape == (0, 5, 144)
+    back = eng.dequantize(*cache, slots=slots, channel_major=channel_major, out=torch.full_like(x, 3.0))
+    assert back.shape == x.shape and not bool(back.any())

@@ -360,6 +360,8 @@ class PoseEngine:
         self._counts('dequantize', n_images, rows, c, n_slots)
         if out is None:
             out = self._empty(shape, dtype)
+        elif not isinstance(out, torch.Tensor):
+            raise TypeError('out: expected a torch tensor')
         kind = self._DTYPES.get(out.dtype)
         if kind is None:
             raise TypeError(f'dtype: float32, bfloat16 or float16, got {out.dtype}')
@@ -374,6 +376,8 @@ class PoseEngine:
         """The result's tensor, address and type; a fresh one is zero where `fill` says that not all of it is written."""
         if out is None:
             out = (torch.zeros if fill else torch.empty)(shape, dtype=dtype, device=self.device)
+        elif not isinstance(out, torch.Tensor):
+            raise TypeError('out: expected a torch tensor')
         elif out.shape != shape:
             raise ValueError(f'out: expected {tuple(shape)}, got {tuple(out.shape)}')
         if out.dtype is not torch.float32 and out.dtype is not torch.bfloat16:
@@ -404,7 +408,7 @@ class PoseEngine:
         bank_at, n_banks = self._offsets(bank_offsets, 'bank_offsets', N)
         of_at = self._index(bank_of, 'bank_of', n_seg, n_banks)
         if n_cols is None:
-            n_cols = out.shape[1] if out is not None and out.dim() == 2 else N
+            n_cols = out.shape[1] if isinstance(out, torch.Tensor) and out.dim() == 2 else N
         self._counts('q8_grouped_product', n_seg, N, n_banks, K, int(n_cols))
         out, at, kind = self._product_out(out, (M, int(n_cols)), dtype, True)
         self._done(self.lib.nemo_q8_grouped_product(self.ctx, ac, ae, M, row_at, n_seg, bc, be, N, bank_at, n_banks, of_at, K, kind, out.shape[1], at,

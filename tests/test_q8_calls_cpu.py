@@ -1,5 +1,6 @@
 """PoseEngine's 8-bit calls on the CPU: what they hand to the library, and what they refuse before it.  Tensors are on the meta device
 (shapes without memory), the library is a list of calls."""
+import numpy as np
 import pytest
 import torch
 
@@ -81,3 +82,18 @@ def test_sizes_reach_the_library_whole(eng):
     got = [(name[5:], a[3:7] + a[8:9] if name == 'nemo_quantize' else a[4:8] if name == 'nemo_dequantize' else (a[3],) + a[6:8]) for name, a in eng.lib.calls]
     assert got == [('quantize', (False, 1, 105, 48, 1)), ('quantize', (True, 3, 35, 48, 3)), ('quantize', (False, 3, 35, 48, 9)),
                    ('dequantize', (1, 1, 45, 48)), ('dequantize', (9, 9, 5, 48)), ('dequantize', (9, 4, 5, 48)), ('q8_product', (LOW, 3, 16))]
+
+
+def test_what_is_no_tensor_is_refused(eng):
+    q, b = held(1, 1, 1, 128), held(4, 128)
+    for bad in ([1.0], np.zeros((4, 128), np.float32), 'out', 3):
+        for call in (lambda: eng.quantize(bad), lambda: eng.quantize(meta(4, 128), out=bad), lambda: eng.quantize(meta(4, 128), out=(bad, bad)),
+                     lambda: eng.quantize(meta(4, 128), slots=bad, out=b), lambda: eng.dequantize(bad, bad), lambda: eng.dequantize(*b, slots=bad),
+                     lambda: eng.dequantize(*b, out=bad), lambda: eng.q8_product(bad, b), lambda: eng.q8_product(b, b, out=bad),
+                     lambda: eng.q8_grouped_product(b, bad, b, index(2)), lambda: eng.q8_grouped_product(b, index(2), b, bad),
+                     lambda: eng.q8_grouped_product(b, index(2), b, index(2), bank_of=bad), lambda: eng.q8_grouped_product(b, index(2), b, index(2), out=bad),
+                     lambda: eng.q8_clutter_score(bad, b), lambda: eng.q8_clutter_score(q, b, bad), lambda: eng.q8_clutter_score(q, b, index(2), bad),
+                     lambda: eng.q8_clutter_score(q, b, out=bad)):
+            with pytest.raises(TypeError):
+                call()
+    assert eng.lib.calls == []

@@ -229,7 +229,7 @@ class BatchPoseSolver:
         eng = self.engine
         if isinstance(feats, q8.Q8):
             if clutter8 and not self.cfg.turn_off_clutter and clutter_scores is None:
-                clutter_scores = eng.q8_clutter_score(feats, eng.quantize(clutter.reshape(-1, eng.D).contiguous()))
+                clutter_scores = eng.q8_clutter_score(feats, eng.quantize((clutter[None] if clutter.dim() == 1 else clutter).contiguous()))
             feats = eng.dequantize(*feats)
         if self.cfg.turn_off_clutter:
             clu = None

@@ -81,3 +81,20 @@ def test_runner_keeps_the_clutter_vectors_of_a_record_in_8_bits(tmp_path):
             # the vector itself is computed in fp32 by the solver: 8 steps of it (mean, square, sum, root, quotient)
             off = (info['clu'][i].cpu().double() - score).abs()
             assert bool((off <= bound + 8 * 2.0 ** -23 * bound / (129 * 2.0 ** -23)).all())
+
+
+def test_solver_refuses_clutter_vectors_of_another_length():
+    """As with f32 maps: [K, D] or [D], and nothing that could be folded into that."""
+    from nemo_amd.pose_solver import SolverConfig
+    from nemo_amd.workloads import twelve_class_workload
+    wl = twelve_class_workload(2, seed=9, cfg=SolverConfig(image_size=(256, 384), total_epochs=5), categories=['car'])
+    s, eng = wl.solver, wl.solver.engine
+    maps = eng.quantize(wl.feats)
+    for shape in ((2, 256), (1, 2, 128), (256,), (256, 64)):
+        for feats, c8 in ((maps, True), (maps, False), (wl.feats, True)):
+            with pytest.raises(ValueError):
+                s.solve_all(feats, torch.ones(shape, device='cuda'), wl.mesh_idx, clutter8=c8)
+    vec = torch.nn.functional.normalize(torch.ones(1, 128)).cuda()
+    for c8 in (True, False):
+        a, b = s.solve_all(maps, vec, wl.mesh_idx, clutter8=c8), s.solve_all(maps, vec[0], wl.mesh_idx, clutter8=c8)
+        assert torch.equal(a.campos, b.campos) and torch.equal(a.loss, b.loss)

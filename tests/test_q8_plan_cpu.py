@@ -4,7 +4,7 @@ import random
 
 import pytest
 
-from tests import q8_plan
+from tests import q8_plan, q8_reach
 from tests.q8_plan import FEW, FITS, LONG, SHORT, WIDE, plan
 
 
@@ -65,3 +65,16 @@ def test_rows_are_counted_in_an_int():
     assert 7 * 4 * 32 + 3 * 32 + 31 == 1023 and top - 1 + 1023 < 2 ** 31
     for n, fits in ((top, 1), (top + 1, 0), (2 ** 31 - 1, 0), (2 ** 31, 0), (2 ** 32 + 1, 0), (2 ** 40, 0)):
         assert lib.rows_fit(ctypes.c_int64(n)) == fits
+
+
+def test_sizes_of_the_gpu_tests_reach_each_kernel():
+    for sizes, kernel in ((q8_reach.FEW, FEW), (q8_reach.SHORT, SHORT), (q8_reach.LONG, LONG)):
+        for m, n, k in sizes:
+            for out_bytes in (2, 4):
+                assert plan(m, n, k, out_bytes).kernel == kernel, (m, n, k)
+    assert {plan(*s).split for s in q8_reach.FEW} == {0, 1} and {plan(*s).across for s in q8_reach.FEW} == {1, 4}
+    assert any(k % 128 for _, _, k in q8_reach.SHORT) and any(k % 128 for _, _, k in q8_reach.LONG)
+    # the score: 256-pixel workgroups from half the compute units on
+    for sizes, lds in ((q8_reach.SCORES_FEW, False), (q8_reach.SCORES_LDS, True)):
+        for n, h, w, d in sizes:
+            assert (2 * n * -(-h * w // 256) >= 256) == lds

@@ -281,6 +281,8 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
  * cores: features against a vertex or clutter bank, or the 1x1 convolution behind a backbone.  The numbers are exact in bf16, but for the
  * ends of its range: here and below, numbers under 2^-133 in size (scale bytes 0 to 2; quantising writes 10 at least) are rounded to
  * multiples of it, and 2^128 or more is infinity, as it reads back (times zero: NaN).
+ * The same call gives the same bits every time.  Up to 256 channels a row's products and scores do not depend on the rows and columns beside it
+ * either; beyond, their number chooses the order in which the blocks of 128 are added.
  * Here and below, a and b have up to 2^31 - 1024 rows, and rows of the result up to 2^27 numbers (here N, below n_cols);
  * NEMO_ERR_UNSUPPORTED beyond, and where a launch does not hold the results (one segment of up to 2^30 - 1024 rows: none that fits 288 GB). */
 int nemo_q8_product(nemo_ctx *ctx, const uint8_t *d_a, const uint8_t *d_ae, int64_t M, const uint8_t *d_b, const uint8_t *d_be,

@@ -302,17 +302,13 @@ class PoseEngine:
                 raise ValueError(f'{name}: must rise from 0 or more to at most {end}')
         return at, t.shape[0] - 1
 
+    # Sizes go to the library as int32, which would drop their upper bits without a word: the calls compare what all of them have set.
     @staticmethod
-    def _counts(what, *counts):
-        """Sizes that go to the library as int32, which would drop their upper bits without a word."""
-        if max(counts) > 0x7fffffff:
-            raise ValueError(f'{what}: more than 2^31 - 1 of a size: {counts}')
-
-    def _done(self, rc, what):
-        if rc < 0:
-            _lib.check(self.ctx, rc, what)
+    def _too_large(what, *counts):
+        raise ValueError(f'{what}: more than 2^31 - 1 of a size: {counts}')
 
     _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _RESULTS = {torch.float32: 0, torch.bfloat16: 1}
 
     def quantize(self, x, channel_major=False, slots=None, out=None):
         """nemo_quantize: rows of f32, bf16 or f16 numbers to q8.Q8(codes, scale), channels last.  x is [..., C], or [n, C, ...]
@@ -336,10 +332,12 @@ class PoseEngine:
         slot_at = self._index(slots, 'slots', n, n_slots)
         if slots is None and not channel_major:   # one run of rows
             n, rows, n_slots = 1, n * rows, 1
-        self._counts('quantize', n, rows, c, n_slots)
-        self._done(self.lib.nemo_quantize(self.ctx, at, dtype, channel_major, n, rows, c, slot_at, n_slots, codes, scale, self._raw_stream()),
-                   'nemo_quantize')
-        return q8.Q8(*out)
+        if n | rows | c | n_slots > 0x7fffffff:
+            self._too_large('quantize', n, rows, c, n_slots)
+        rc = self.lib.nemo_quantize(self.ctx, at, dtype, channel_major, n, rows, c, slot_at, n_slots, codes, scale, self._raw_stream())
+        if rc < 0:
+            _lib.check(self.ctx, rc, 'nemo_quantize')
+        return out if type(out) is q8.Q8 else q8.Q8(*out)
 
     def dequantize(self, codes, scale, slots=None, channel_major=False, dtype=torch.float32, out=None):
         """nemo_dequantize: rows held in 8 bits back to numbers of `dtype` (of `out`, where that is given): all of them, or the images slots[i]
@@ -357,7 +355,8 @@ class PoseEngine:
         rows, n_images, n_slots = math.prod(image), n, room[0]
         if slots is None and not channel_major:   # one run of rows
             n_images, rows, n_slots = 1, n * rows, 1
-        self._counts('dequantize', n_images, rows, c, n_slots)
+        if n_images | rows | c | n_slots > 0x7fffffff:
+            self._too_large('dequantize', n_images, rows, c, n_slots)
         if out is None:
             out = self._empty(shape, dtype)
         elif not isinstance(out, torch.Tensor):
@@ -368,8 +367,10 @@ class PoseEngine:
         at = self._ready(out, out.dtype, 'out')
         if out.shape != shape:
             raise ValueError(f'out: expected {tuple(shape)}, got {tuple(out.shape)}')
-        self._done(self.lib.nemo_dequantize(self.ctx, codes_at, scale_at, slot_at, n_slots, n_images, rows, c, kind, channel_major, at,
-                                            self._raw_stream()), 'nemo_dequantize')
+        rc = self.lib.nemo_dequantize(self.ctx, codes_at, scale_at, slot_at, n_slots, n_images, rows, c, kind, channel_major, at,
+                                      self._raw_stream())
+        if rc < 0:
+            _lib.check(self.ctx, rc, 'nemo_dequantize')
         return out
 
     def _product_out(self, out, shape, dtype, fill):
@@ -380,9 +381,10 @@ class PoseEngine:
             raise TypeError('out: expected a torch tensor')
         elif out.shape != shape:
             raise ValueError(f'out: expected {tuple(shape)}, got {tuple(out.shape)}')
-        if out.dtype is not torch.float32 and out.dtype is not torch.bfloat16:
+        kind = self._RESULTS.get(out.dtype)
+        if kind is None:
             raise TypeError(f'out: float32 or bfloat16, got {out.dtype}')
-        return out, self._ready(out, out.dtype, 'out'), self._DTYPES[out.dtype]
+        return out, self._ready(out, out.dtype, 'out'), kind
 
     def q8_product(self, a, b, dtype=torch.float32, out=None):
         """nemo_q8_product: [..., K] times [N, K] -> [..., N], both (codes, scale); f32 or bf16."""
@@ -390,9 +392,12 @@ class PoseEngine:
         bshape, bc, be = self._q8(b, 'b')
         if len(bshape) != 2 or bshape[1] != k:
             raise ValueError(f'b: expected [N, {k}], got {tuple(bshape)}')
-        self._counts('q8_product', bshape[0], k)
+        if bshape[0] | k > 0x7fffffff:
+            self._too_large('q8_product', bshape[0], k)
         out, at, kind = self._product_out(out, (*m, bshape[0]), dtype, False)
-        self._done(self.lib.nemo_q8_product(self.ctx, ac, ae, math.prod(m), bc, be, bshape[0], k, kind, at, self._raw_stream()), 'nemo_q8_product')
+        rc = self.lib.nemo_q8_product(self.ctx, ac, ae, math.prod(m), bc, be, bshape[0], k, kind, at, self._raw_stream())
+        if rc < 0:
+            _lib.check(self.ctx, rc, 'nemo_q8_product')
         return out
 
     def q8_grouped_product(self, a, row_offsets, b, bank_offsets, bank_of=None, n_cols=None, dtype=torch.float32, out=None):
@@ -409,10 +414,14 @@ class PoseEngine:
         of_at = self._index(bank_of, 'bank_of', n_seg, n_banks)
         if n_cols is None:
             n_cols = out.shape[1] if isinstance(out, torch.Tensor) and out.dim() == 2 else N
-        self._counts('q8_grouped_product', n_seg, N, n_banks, K, int(n_cols))
-        out, at, kind = self._product_out(out, (M, int(n_cols)), dtype, True)
-        self._done(self.lib.nemo_q8_grouped_product(self.ctx, ac, ae, M, row_at, n_seg, bc, be, N, bank_at, n_banks, of_at, K, kind, out.shape[1], at,
-                                                    self._raw_stream()), 'nemo_q8_grouped_product')
+        n_cols = int(n_cols)
+        if n_seg | N | n_banks | K | n_cols > 0x7fffffff:
+            self._too_large('q8_grouped_product', n_seg, N, n_banks, K, n_cols)
+        out, at, kind = self._product_out(out, (M, n_cols), dtype, True)
+        rc = self.lib.nemo_q8_grouped_product(self.ctx, ac, ae, M, row_at, n_seg, bc, be, N, bank_at, n_banks, of_at, K, kind, out.shape[1], at,
+                                              self._raw_stream())
+        if rc < 0:
+            _lib.check(self.ctx, rc, 'nemo_q8_grouped_product')
         return out
 
     def q8_clutter_score(self, feat, cbank, bank_offsets=None, bank_of=None, out=None):
@@ -427,12 +436,14 @@ class PoseEngine:
             raise ValueError(f'cbank: expected [K, {self.D}], got {tuple(bshape)}')
         n, (bank_at, n_banks) = fshape[0], (None, 1) if bank_offsets is None else self._offsets(bank_offsets, 'bank_offsets', bshape[0])
         of_at = self._index(bank_of, 'bank_of', n, n_banks)
-        self._counts('q8_clutter_score', n, bshape[0], n_banks)
+        if n | bshape[0] | n_banks > 0x7fffffff:
+            self._too_large('q8_clutter_score', n, bshape[0], n_banks)
         out, at, kind = self._product_out(out, (n, self.h, self.w), torch.float32, bank_of is not None)
         if kind:
             raise TypeError('out: expected torch.float32')
-        self._done(self.lib.nemo_q8_clutter_score(self.ctx, fc, fe, n, bc, be, bshape[0], bank_at, n_banks, of_at, at, self._raw_stream()),
-                   'nemo_q8_clutter_score')
+        rc = self.lib.nemo_q8_clutter_score(self.ctx, fc, fe, n, bc, be, bshape[0], bank_at, n_banks, of_at, at, self._raw_stream())
+        if rc < 0:
+            _lib.check(self.ctx, rc, 'nemo_q8_clutter_score')
         return out
 
     def score_fwd_bwd(self, feat, clu, C_, theta, img_idx=None, mesh_idx=None, want_grad=True):

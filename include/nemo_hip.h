@@ -269,7 +269,8 @@ int nemo_solve_static(nemo_ctx *ctx, int32_t N, const int32_t *d_img_idx, const 
 /* Writes n images of `rows` pixels into a cache of n_slots images: image i to slot d_slots[i] (NULL: slot i).  d_x is of `dtype`
  * [n][rows][C], or [n][C][rows] with channel_major (what a backbone leaves and a feature record holds).  d_q u8[n_slots][rows][C],
  * d_e u8[n_slots][rows][ceil(C / 128)].  An image whose slot is outside [0, n_slots) is not written; of several images
- * with the same slot the last one stays; slots that no image names are left as they were.  Plain rows (a bank): n = 1, rows = their number. */
+ * with the same slot the last one stays; slots that no image names are left as they were.  Plain rows (a bank): n = 1, rows = their number.
+ * With d_slots every image looks at the slots of those behind it, n^2 / 2 of them in all: beyond some 10^4 images of a few pixels that is most of the call. */
 int nemo_quantize(nemo_ctx *ctx, const void *d_x, int32_t dtype, int32_t channel_major, int32_t n, int32_t rows, int32_t C,
                   const int32_t *d_slots, int32_t n_slots, uint8_t *d_q, uint8_t *d_e, void *stream);
 /* Reads images back: slot d_slots[i] (NULL: slot i) to image i of d_x, of `dtype` and layout as above, rounded once to `dtype` (a number

@@ -78,7 +78,8 @@ __device__ __forceinline__ int q8_slot(const int32_t *slots, int i, int n_slots)
   return s >= 0 && s < n_slots ? s : -1;
 }
 // Two images written to the same slot: the later one stays, as if they were written in order.  Whether a later image
-// than i has slot s (whole workgroup).
+// than i has slot s (whole workgroup).  Every workgroup reads the slots behind its image's: no matter at 512 images (of 16 pixels x 128, f32:
+// 8.0 us, 7.6 without slots), much at many small ones (16384: 72 and 27 us, 262144: 8.7 and 0.49 ms).
 __device__ __forceinline__ bool q8_overwritten(const int32_t *slots, int i, int n, int s) {
   if (!slots) return false;
   bool hit = false;
@@ -699,8 +700,10 @@ __device__ __forceinline__ void q8_store_group(typename TT::T *out, int ld, int 
 // begin in the middle of one, and waits for no store.  With wc < 8, 8 / wc waves share the columns and take the row tiles in turn; so do
 // all 8 where a bank's last columns are few (262144 rows x 1088: bf16 136 -> 125 us, f32 227 -> 213; x 640 f32 152 -> 134; x 1095, whose lines
 // are shared between the cuts, bf16 182 -> 186, f32 240 -> 242).  f32 reaches 5.2 TB/s of results where rows are whole lines and 4.7 where
-// they are not (x 1095), bf16 4.5 and 3.1: a line that leaves in two parts costs about as much as two (stores alone, without the products,
-// reach 5.4 and 3.2 on the same rows in bf16; a mixed batch of 12 banks into bf16 rows of 1095 takes 158 us, 155 without its products).
+// they are not (x 1095), bf16 4.5 and 3.1: a line that leaves in two parts costs about as much as two (these stores without the products
+// reach 5.4 and 3.2 on the same rows in bf16, a linear fill of either result 6.9).  A mixed batch of 12 banks of 536 to 1095 rows into bf16 rows
+// of 1095 takes 158-168 us for 421 MB, 155 without its products: an XCD has one contiguous eighth of all row tiles and cuts, which hold
+// 0.77 to 1.25 of the mean of results there, and the rows begin inside lines; with 12 banks of 1024 it takes 128 us for 574 MB.
 // Twice the columns a wave, so that a bf16 row leaves in the same 256 bytes as an f32 one, takes 216 registers and leaves one workgroup a compute
 // unit: 200 us for 262144 x 1095, 250 for the mixed batch.
 template <class TT, bool TAIL>

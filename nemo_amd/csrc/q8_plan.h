@@ -46,9 +46,14 @@ inline Q8Plan q8_plan(const Q8Problem &p) {
   }
   const size_t chunks = ((size_t)p.n_cols + 127) / 128, cus = (size_t)p.n_cu;
   const int nb = (p.K + 127) / 128;
-  // Up to 32 columns, or so few rows that 32 x 128 products a workgroup make at most 3 workgroups for 2 compute units, or fewer than 64 rows a
-  // segment: one wave for 32 x 32 (f32 results: 1000 x 1000 x 128 4.3 us that way, 5.9 and 5.7 with the kernels below; 300 x 8000 x 128
-  // 7.1, 6.5 and 6.1; 262144 x 16 x 128 11.5, 21.5 and 20.7).  The others take what does not fit its grid.
+  // One wave for 32 x 32 in three cases (f32 results, us; in brackets with the kernels below, which also take what does not fit its grid):
+  // - Up to 32 columns: 262144 x 16 x 128 10.8 (18.8), x 32 12.3 (19.1), x 48 21.8 (19.8); x 16 x 512 36.6 (42.5), x 32 39.2 (45.3), x 48 69.8
+  //   (47.5); 100000 x 32 x 2048 46.9 (63.1), x 48 76.3 (64.8).
+  // - So few rows that 32 x 128 products a workgroup make at most 3 workgroups for 2 compute units: 1000 x 1000 x 128 on the device alone 4.3 (5.7),
+  //   300 x 8000 x 128 7.1 (6.1).
+  // - Fewer than 64 rows a segment on average: 256 segments of 8 x 1000 x 128 15.2 (16.4), of 32 17.6 (19.9), of 48 26.2 (23.9), of 64 33.7 (31.6).
+  //   What it does not see: with K = 512 it loses at any length (of 8 49.9 (43.4), of 48 95.5 (54.5)), and where most segments are empty
+  //   (12 of 2000 rows among 600 x 128 52 (67), but among 3000 319 (195), x 512 1198 (356)).
   if (p.n_cols <= 32 || 2 * q8_tiles(p, 32) * chunks <= 3 * cus || (size_t)p.M < 64 * (size_t)p.n_seg) {
     r.kernel = Q8_FEW;
     r.split = nb > 2;

@@ -169,8 +169,11 @@ class FeatureRecord:
             done += n
 
     def read_feature8_into(self, name: str, codes: np.ndarray, scale: np.ndarray, fd: int) -> None:
-        """Fill `codes` (u8, h w D bytes) and `scale` (u8) with the map `name` of an 8-bit record: one read, or the zip reader
-        where the record is compressed."""
+        """Fill `codes` (u8, C-contiguous, h w D bytes) and `scale` (u8 likewise) with the map `name` of an 8-bit record: one read, or the
+        zip reader where the record is compressed."""
+        for part, n in zip((codes, scale), self._size8()):
+            if part.dtype != np.uint8 or part.size != n or not part.flags.c_contiguous:   # a copy would be filled in its place
+                raise ValueError('read_feature8_into: expected %d contiguous bytes, got %s %s' % (n, part.dtype, part.shape))
         lay = self._layout(name)
         if lay is None:
             f = self.feature8(name)
@@ -375,6 +378,8 @@ def write_feature_record8(path: str, memory: Dict[str, np.ndarray], clutter: Dic
         if f.codes.dim() != 3 or tuple(f.codes.shape) != (shape or tuple(f.codes.shape)) or \
                 tuple(f.scale.shape) != tuple(f.codes.shape[:2]) + (q8.n_blocks(f.codes.shape[2]),):
             raise ValueError('map %r: expected [h, w, D] of one shape, got %s' % (n, tuple(f.codes.shape)))
+        if f.codes.dtype != torch.float8_e4m3fn or f.scale.dtype != torch.float8_e8m0fnu:
+            raise ValueError('map %r: expected codes and scales, got %s and %s' % (n, f.codes.dtype, f.scale.dtype))
         shape = tuple(f.codes.shape)
         get[n] = np.concatenate([v.detach().cpu().contiguous().view(torch.uint8).numpy().reshape(-1) for v in f])
     if shape is None:

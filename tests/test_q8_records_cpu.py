@@ -122,3 +122,22 @@ def test_directory_of_a_record_leaves_no_file_open(tmp_path, monkeypatch):
     assert open_files() == kept
     r.close()
     assert open_files() == before
+
+
+def test_record_takes_and_fills_what_it_names(tmp_path):
+    """Maps of other types are not written as if they were codes, and buffers that a read would not reach are refused."""
+    a = q8.quantize_host(torch.ones(4, 5, 128))
+    dst = tmp_path / 'q8.npz'
+    for bad in (q8.Q8(a.codes.float(), a.scale), q8.Q8(a.codes, a.scale.float()), q8.Q8(a.codes.view(torch.uint8), a.scale.view(torch.uint8))):
+        with pytest.raises(ValueError, match='expected codes and scales'):
+            records.write_feature_record8(str(dst), {}, {}, {}, {'a': bad})
+    assert not dst.exists()
+    records.write_feature_record8(str(dst), {}, {}, {}, {'a': a})
+    codes, scale = np.zeros((4, 5, 128), np.uint8), np.zeros((4, 5, 1), np.uint8)
+    with records.FeatureRecord(str(dst)) as r, open(dst, 'rb') as fh:
+        r.read_feature8_into('a', codes, scale, fh.fileno())
+        assert np.array_equal(codes, a.codes.view(torch.uint8).numpy()) and np.array_equal(scale, a.scale.view(torch.uint8).numpy())
+        for c, s in ((codes.transpose(1, 0, 2), scale), (codes[:, ::2], scale), (codes.view(np.int8), scale), (codes[:3], np.zeros((4, 5, 33), np.uint8)),
+                     (codes, scale[:, :, [0, 0]]), (codes, np.zeros((4, 5), np.float32))):
+            with pytest.raises(ValueError, match='contiguous bytes'):
+                r.read_feature8_into('a', c, s, fh.fileno())

@@ -1215,7 +1215,7 @@ int nemo_dequantize(nemo_ctx *ctx, const uint8_t *d_q, const uint8_t *d_e, const
   const int nb = (C + Q8_BLOCK - 1) / Q8_BLOCK;
   const size_t per = channel_major ? ((size_t)rows + 255) / 256 : ((size_t)rows * (C / (dtype == NEMO_F32 ? 4 : 8)) + 256 * Q8_DU - 1) / (256 * Q8_DU);
   const size_t image = per * (channel_major ? nb : 1), blocks = image * n;
-  if (image > Q8_MAX_BLOCKS || blocks > Q8_MAX_BLOCKS - 7)  // channels first: blocks are rounded up to whole eights
+  if (image > Q8_MAX_BLOCKS || blocks > Q8_MAX_BLOCKS - (channel_major ? 7 : 0))  // channels first: they are rounded up to whole eights
     return fail(ctx, NEMO_ERR_UNSUPPORTED, "nemo_dequantize: too many rows for one launch");
   DeviceGuard on(ctx->device);
   HIP_TRY(ctx, on.status);
